@@ -99,6 +99,31 @@ typedef struct nnc_hip_kv nnc_hip_kv;
 nnc_status nnc_hip_kv_create(int32_t n_buf, const int32_t* rows, const int32_t* kv_dim, bool bf16,
                              nnc_hip_kv** out);
 
+/* As nnc_hip_kv_create, K and V held in 4 bits: 5 bits an element with the
+ * scales, 0.31 of BF16's bytes. No counterpart in nnc, whose caches are BF16
+ * and F32. A block is 32 consecutive elements of a row, nnc's own 4-bit weight
+ * block (reference nn_ops.h:138-142) along the head: with lo and hi its least
+ * and largest element,
+ *   s = f16((hi - lo) / 15), z = f16(lo), c = rint((x - z) / s) in 0 .. 15
+ * (0 where s is 0), and x is held as f16(c * s + z), rounded once. Elements
+ * are brought within +-65280 first and a NaN is held as 0, so every value of
+ * such a cache is finite. The other calls take it as they take the others:
+ *   nnc_hip_kv_append_f32, _f32_device and nnc_hip_kv_prep_append_device
+ *     quantise on the device (rows in device memory 16-byte aligned);
+ *   nnc_hip_kv_append and nnc_hip_kv_read move rows in an interchange form:
+ *     per block s and z (FP16), then 16 bytes, elements i and i + 16 of the
+ *     block in the low and the high half of byte i: kv_dim / 32 * 20 bytes a
+ *     row. Blocks with |z| + 15 |s| past FP16's range, infinite or NaN are
+ *     refused (NNC_ERR_INVALID_ARGUMENT);
+ *   the attend calls compute over the values that the cache holds, with the
+ *     error of fp32 sums; head_dim 32, 64, 96, 128, 192, 256 or 512 (else
+ *     NNC_ERR_UNSUPPORTED_MODEL), any group up to 16. No limit on a buffer's
+ *     bytes. Batches of up to 16 tokens, and every batch in exact mode, give
+ *     each token the bits of its one-token call, as over the other caches.
+ * NNC_ERR_INVALID_ARGUMENT also for rows or kv_dim that are no multiples of
+ * 32 (round n_ctx up; rings are multiples of 256). */
+nnc_status nnc_hip_kv_create_q4(int32_t n_buf, const int32_t* rows, const int32_t* kv_dim, nnc_hip_kv** out);
+
 /* Frees the buffers, the scratch and the stream. NULL is a no-op. */
 void nnc_hip_kv_free(nnc_hip_kv* kv);
 
@@ -189,6 +214,12 @@ nnc_status nnc_hip_kv_prep_append_device(nnc_hip_kv* kv, int32_t buf, int32_t po
 /* Copies rows row0 .. row0 + n_rows - 1 of buffer `buf` (raw element bits)
  * to host memory and waits. Either output may be NULL. */
 nnc_status nnc_hip_kv_read(nnc_hip_kv* kv, int32_t buf, int32_t row0, int32_t n_rows, void* k_out, void* v_out);
+
+/* The values of rows row0 .. row0 + n_rows - 1 of buffer `buf` as F32 rows of
+ * kv_dim in device memory (16-byte aligned), whatever the cache's element
+ * type. Either output may be NULL. Asynchronous on the cache's stream. */
+nnc_status nnc_hip_kv_read_f32_device(nnc_hip_kv* kv, int32_t buf, int32_t row0, int32_t n_rows, float* k_out,
+                                      float* v_out);
 
 /* The attention core of attention_forward (reference model.cpp:1693-1761)
  * for one layer whose K/V live in buffer `buf`:

@@ -1,0 +1,315 @@
+// Split-K attention over the 4-bit cache (kv_q4.h): decode and session batches,
+// and every batch in exact mode.
+//
+// S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_16x16x32_f16, the keys' values as
+// the format defines them (fp16, exact), Q and P as fp16 hi + lo: 22 significant
+// bits, so scores and outputs have the error of fp32 sums. A product's 16
+// columns are 8 (token, query head) pairs, their hi parts in columns 0 .. 7 and
+// their lo parts in columns 8 .. 15; one rotation by half a row adds the two.
+// Every pair goes through the same instructions in whatever column and batch it
+// lies, and a group of keys outside its span changes nothing in it (weights
+// exactly 0, factors exactly 1), so a token's bits depend on its own split grid
+// alone.
+//
+// A work-group of four wavefronts owns one KV head, one range of keys and T
+// columns tiles of 8 pairs; its wavefronts take groups of 32 keys in turn
+// (record by record, straight into operand registers), keep running maxima and
+// sums of their own, and meet in LDS at the end.
+#include "kernels.h"
+#include "kv_q4.h"
+
+#include <type_traits>
+
+namespace nnchip
+{
+	namespace
+	{
+		constexpr int kW = kQ4Waves;
+		// A pair's weights are 2^(score - offset). The offset is raised, to kBelow
+		// under the largest score so far, when a score passes it by more than kRaise:
+		// weights stay under 2^kRaise (fp16 holds them) and a pair's largest weight is
+		// at least 2^kBelow, so the steps of fp16's lo part (2^-25 at the least) are
+		// 2^-31 of it.
+		constexpr float kRaise = 14.0f, kBelow = 6.0f;
+
+		__device__ __forceinline__ float ror8(float x)
+		{
+			return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
+		}
+		__device__ __forceinline__ float max_other_row(float x)
+		{
+			const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+			return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+		}
+		// Over the four lanes of a column.
+		__device__ __forceinline__ float column_max(float x) { return max_with_other_half(max_other_row(x)); }
+		__device__ __forceinline__ float column_sum(float x) { return add_with_other_half(add_with_other_row(x)); }
+
+		// One record's registers: 32 rows, 32 columns of K and V.
+		struct record
+		{
+			u32x4 code;
+			u32x2 ksz;
+			u32x4 vs, vz;
+		};
+
+		__device__ __forceinline__ record load_record(const unsigned char* rec, int lane)
+		{
+			record r;
+			r.code = load_stream(rec + 16 * lane);
+			r.ksz = *reinterpret_cast<const u32x2*>(rec + kQ4KScales + 8 * (lane & 15));
+			r.vs = *reinterpret_cast<const u32x4*>(rec + kQ4VScales + 32 * (lane >> 4));
+			r.vz = *reinterpret_cast<const u32x4*>(rec + kQ4VScales + 32 * (lane >> 4) + 16);
+			return r;
+		}
+
+		// hi (is_lo false) or lo part of two weights.
+		__device__ __forceinline__ uint32_t part_of(float a, float b, bool is_lo)
+		{
+			const f16x2 h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+			const f16x2 l = {static_cast<_Float16>(a - static_cast<float>(h.x)), static_cast<_Float16>(b - static_cast<float>(h.y))};
+			return as_u32(is_lo ? l : h);
+		}
+
+		template <int NB, int T>
+		__global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(1, 2))) void decode_q4_kernel(
+			const decode_params p, int group)
+		{
+			constexpr int HD = NB * kQ4Block;
+			const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+			const int split = blockIdx.x, kvh = blockIdx.y;
+			const int c8 = lane & 7, g = lane >> 4;
+			const bool is_lo = (lane & 8) != 0;
+			const int n_pairs = p.n_tok * group;
+
+			__shared__ float s_o[kW][8][HD + 4]; // a tile's outputs (relative to its offset), offset, sum
+
+			// Q: per pair brought under 2^15 by a power of two, then fp16 hi or lo.
+			f16x8 q[T][NB];
+			float back[T]; // 2^-that power, and log2(e) * scale
+			int first[T], last[T];
+#pragma unroll
+			for (int i = 0; i < T; ++i)
+			{
+				const int pair = (blockIdx.z * T + i) * 8 + c8;
+				const bool real = pair < n_pairs;
+				const int tok = real ? pair / group : 0, h = real ? pair % group : 0;
+				attn_span(p.causal, p.window, p.pos0 + tok, p.n_seq, first[i], last[i]);
+				if (!real) last[i] = -1, first[i] = 0;
+				const float* src = p.q + (static_cast<size_t>(tok) * p.n_head + kvh * group + h) * HD + 8 * g;
+				float x[NB][8];
+				float m = 0.0f;
+#pragma unroll
+				for (int b = 0; b < NB; ++b)
+				{
+					const float4 u = *reinterpret_cast<const float4*>(src + 32 * b), v = *reinterpret_cast<const float4*>(src + 32 * b + 4);
+					// k slot order: columns 0, 4, 1, 5, 2, 6, 3, 7
+					x[b][0] = u.x, x[b][1] = v.x, x[b][2] = u.y, x[b][3] = v.y;
+					x[b][4] = u.z, x[b][5] = v.z, x[b][6] = u.w, x[b][7] = v.w;
+#pragma unroll
+					for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[b][j]));
+				}
+				m = column_max(m);
+				// (0, infinity and NaN: as they are)
+				const int e = m > 0.0f && m < INFINITY ? 14 - ilogbf(m) : 0;
+				back[i] = ldexpf(p.qscale, -e);
+#pragma unroll
+				for (int b = 0; b < NB; ++b)
+				{
+					u32x4 w;
+#pragma unroll
+					for (int j = 0; j < 4; ++j) w[j] = part_of(ldexpf(x[b][2 * j], e), ldexpf(x[b][2 * j + 1], e), is_lo);
+					q[i][b] = as_f16x8(w);
+				}
+			}
+
+			f32x4 o[T][NB][2] = {};
+			float m_off[T], l[T];
+#pragma unroll
+			for (int i = 0; i < T; ++i) m_off[i] = -INFINITY, l[i] = 0.0f;
+
+			// The keys any pair of the launch attends to, within the split.
+			int kmin, kmax, unused;
+			attn_span(p.causal, p.window, p.pos0, p.n_seq, kmin, unused);
+			attn_span(p.causal, p.window, p.pos0 + p.n_tok - 1, p.n_seq, unused, kmax);
+			const int k0 = p.split_base + split * p.split_keys;
+			const int g_first = (kmin > k0 ? kmin : k0) / kQ4Rows;
+			const int g_last = (kmax < k0 + p.split_keys - 1 ? kmax : k0 + p.split_keys - 1) / kQ4Rows;
+			const int row_groups = p.rows / kQ4Rows, blocks = p.kv_dim / kQ4Block;
+			const unsigned char* recs = static_cast<const unsigned char*>(p.K) + static_cast<size_t>(kvh) * NB * kQ4Record;
+			const size_t group_bytes = static_cast<size_t>(blocks) * kQ4Record;
+			// (wavefront w takes the groups whose number in the split is w modulo kW)
+			int kg = k0 / kQ4Rows + wave;
+			if (kg < g_first) kg += (g_first - kg + kW - 1) / kW * kW;
+
+			// Up to 8 blocks the next group's records are in flight during the work on
+			// this one; 16 blocks' registers do not fit twice, and they are loaded here.
+			constexpr bool kAhead = NB <= 8;
+			auto records_of = [&](int n, record* r)
+			{
+#pragma unroll
+				for (int b = 0; b < NB; ++b)
+					r[b] = load_record(recs + static_cast<size_t>(n % row_groups) * group_bytes + b * kQ4Record, lane);
+			};
+			record r[NB];
+			if (kAhead && kg <= g_last) records_of(kg, r);
+			for (; kg <= g_last; kg += kW)
+			{
+				record nx[kAhead ? NB : 1];
+				if constexpr (kAhead)
+					records_of(kg + kW <= g_last ? kg + kW : kg, nx);
+				else
+					records_of(kg, r);
+
+				f32x4 s[T][2] = {};
+#pragma unroll
+				for (int b = 0; b < NB; ++b)
+#pragma unroll
+					for (int t = 0; t < 2; ++t)
+					{
+						const f16x8 a = q4_k(t ? r[b].code.y : r[b].code.x, t ? r[b].ksz.y : r[b].ksz.x);
+#pragma unroll
+						for (int i = 0; i < T; ++i) s[i][t] = mfma16x16x32(a, q[i][b], s[i][t]);
+					}
+
+				f16x8 w[T];
+#pragma unroll
+				for (int i = 0; i < T; ++i)
+				{
+					float sc[8]; // tile t, row j: 4 t + j; key 32 kg + 16 t + 4 g + j
+					float m = -INFINITY;
+#pragma unroll
+					for (int j = 0; j < 8; ++j)
+					{
+						const float d = s[i][j >> 2][j & 3];
+						sc[j] = (d + ror8(d)) * back[i];
+						const int key = kg * kQ4Rows + 16 * (j >> 2) + 4 * g + (j & 3);
+						if (key < first[i] || key > last[i]) sc[j] = -INFINITY;
+						m = fmaxf(m, sc[j]);
+					}
+					m = column_max(m);
+					const float was = m_off[i];
+					if (m > was + kRaise) // (the first keys of a span too: was is -inf)
+					{
+						m_off[i] = m - kBelow;
+						const float f = fast_exp2(was - m_off[i]);
+						l[i] *= f;
+#pragma unroll
+						for (int b = 0; b < NB; ++b) o[i][b][0] *= f, o[i][b][1] *= f;
+					}
+					const float off = m_off[i] == -INFINITY ? 0.0f : m_off[i];
+#pragma unroll
+					for (int j = 0; j < 8; ++j)
+					{
+						sc[j] = fast_exp2(sc[j] - off);
+						l[i] += sc[j];
+					}
+					u32x4 f;
+#pragma unroll
+					for (int j = 0; j < 4; ++j) f[j] = part_of(sc[j], sc[4 + j], is_lo);
+					w[i] = as_f16x8(f);
+				}
+
+#pragma unroll
+				for (int b = 0; b < NB; ++b)
+#pragma unroll
+					for (int t = 0; t < 2; ++t)
+					{
+						const f16x8 a = q4_v(t ? r[b].code.w : r[b].code.z, r[b].vs, r[b].vz);
+#pragma unroll
+						for (int i = 0; i < T; ++i) o[i][b][t] = mfma16x16x32(a, w[i], o[i][b][t]);
+					}
+				if constexpr (kAhead)
+#pragma unroll
+					for (int b = 0; b < NB; ++b) r[b] = nx[b];
+			}
+
+			// The wavefronts' parts of each tile, joined in wavefront order.
+#pragma unroll
+			for (int i = 0; i < T; ++i)
+			{
+				if (i) __syncthreads();
+				l[i] = column_sum(l[i]);
+#pragma unroll
+				for (int b = 0; b < NB; ++b)
+#pragma unroll
+					for (int t = 0; t < 2; ++t)
+					{
+						float4 v;
+						v.x = o[i][b][t][0] + ror8(o[i][b][t][0]);
+						v.y = o[i][b][t][1] + ror8(o[i][b][t][1]);
+						v.z = o[i][b][t][2] + ror8(o[i][b][t][2]);
+						v.w = o[i][b][t][3] + ror8(o[i][b][t][3]);
+						if (!is_lo) *reinterpret_cast<float4*>(&s_o[wave][c8][32 * b + 16 * t + 4 * g]) = v;
+					}
+				if (lane < 8) s_o[wave][c8][HD] = m_off[i], s_o[wave][c8][HD + 1] = l[i];
+				__syncthreads();
+				for (int x = threadIdx.x; x < 8 * HD; x += 64 * kW)
+				{
+					const int c = x / HD, d = x % HD;
+					const int pair = (blockIdx.z * T + i) * 8 + c;
+					if (pair >= n_pairs) break;
+					float mx = s_o[0][c][HD];
+#pragma unroll
+					for (int v = 1; v < kW; ++v) mx = fmaxf(mx, s_o[v][c][HD]);
+					const float off = mx == -INFINITY ? 0.0f : mx;
+					float acc = 0.0f, sum = 0.0f;
+#pragma unroll
+					for (int v = 0; v < kW; ++v)
+					{
+						const float f = fast_exp2(s_o[v][c][HD] - off);
+						acc = fmaf(s_o[v][c][d], f, acc);
+						sum = fmaf(s_o[v][c][HD + 1], f, sum);
+					}
+					const int tok = pair / group, h = pair % group;
+					if (p.n_split > 1)
+					{
+						float* dst = p.part + (((static_cast<size_t>(tok) * p.n_kv + kvh) * p.n_split + split) * group + h) * (HD + 4);
+						dst[d] = acc;
+						if (d == 0) dst[HD] = mx, dst[HD + 1] = sum;
+					}
+					else
+					{
+						const size_t at = (static_cast<size_t>(tok) * p.n_head + kvh * group + h) * HD + d;
+						p.out[at] = gated(acc * (sum > 0.0f ? 1.0f / sum : 0.0f), p.gate, at);
+					}
+				}
+			}
+		}
+
+		template <int NB>
+		void launch_nb(const decode_params& p, int n_tok, int group, hipStream_t stream)
+		{
+			// Several tiles share a work-group's records as far as the registers go.
+			constexpr int kMost = NB <= 3 ? 4 : NB <= 4 ? 2 : 1;
+			const int tiles = (n_tok * group + 7) / 8;
+			auto run = [&](auto t)
+			{
+				constexpr int T = decltype(t)::value;
+				decode_q4_kernel<NB, T><<<dim3(p.n_split, p.n_kv, (tiles + T - 1) / T), 64 * kW, 0, stream>>>(p, group);
+			};
+			if (tiles == 1 || kMost == 1)
+				run(std::integral_constant<int, 1>());
+			else if (tiles == 2 || kMost == 2)
+				run(std::integral_constant<int, kMost < 2 ? 1 : 2>());
+			else
+				run(std::integral_constant<int, kMost>());
+			if (p.n_split > 1) launch_merge_generic(p, n_tok, NB * kQ4Block, group, stream);
+		}
+	}
+
+	bool launch_decode_q4(const decode_params& p, int n_tok, int head_dim, int group, hipStream_t stream)
+	{
+		switch (head_dim)
+		{
+		case 32: launch_nb<1>(p, n_tok, group, stream); return true;
+		case 64: launch_nb<2>(p, n_tok, group, stream); return true;
+		case 96: launch_nb<3>(p, n_tok, group, stream); return true;
+		case 128: launch_nb<4>(p, n_tok, group, stream); return true;
+		case 192: launch_nb<6>(p, n_tok, group, stream); return true;
+		case 256: launch_nb<8>(p, n_tok, group, stream); return true;
+		case 512: launch_nb<16>(p, n_tok, group, stream); return true;
+		default: return false;
+		}
+	}
+}

@@ -127,6 +127,28 @@ namespace nnchip
 	bool launch_tiled3(const decode_params& p, int n_tok, int head_dim, int group, void* split, int k_lo, int k_hi,
 	                   hipStream_t stream);
 
+	// The 4-bit cache (kv_q4.h): its head sizes, and the split-K kernel over it
+	// (p.K: the records; rows a multiple of 32). A split is a multiple of
+	// kQ4UnitKeys keys; kQ4Waves wavefronts share a work-group's keys, a unit at
+	// a time.
+	constexpr int kQ4UnitKeys = 32, kQ4Waves = 4;
+	__host__ __device__ inline bool q4_head_dim(int head_dim)
+	{
+		return head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 192 ||
+		       head_dim == 256 || head_dim == 512;
+	}
+	bool launch_decode_q4(const decode_params& p, int n_tok, int head_dim, int group, hipStream_t stream);
+	// Rows into the records: F32, or (raw) blocks in the interchange form; and
+	// rows row0 .. row0 + n_rows - 1 out of them, likewise. Either output may be
+	// null.
+	void launch_append_q4(void* recs, const void* k_rows, const void* v_rows, int rows, int kv_dim, int pos0, int n_tok,
+	                      bool raw, hipStream_t stream);
+	void launch_read_q4(const void* recs, void* k_out, void* v_out, int kv_dim, int row0, int n_rows, bool raw,
+	                    hipStream_t stream);
+	// Elements first .. first + n - 1 of a BF16 or F32 buffer as F32.
+	void launch_read_rows(const void* K, const void* V, float* k_out, float* v_out, size_t first, size_t n, bool bf16,
+	                      hipStream_t stream);
+
 	// Tiled MFMA attention for a batch of query tokens.
 	struct prefill_params
 	{

@@ -9,6 +9,7 @@
 // return an nnc_status; no C++ exception crosses the ABI.
 #include "../../include/nnc_hip.h"
 #include "kernels.h"
+#include "kv_q4.h"
 
 #include <hip/hip_runtime.h>
 
@@ -96,7 +97,7 @@ namespace
 
 	struct kv_buffer
 	{
-		void* k = nullptr;
+		void* k = nullptr; // a 4-bit cache: the records of K and V (kv_q4.h), and v null
 		void* v = nullptr; // v_alloc + kVOffset
 		// BF16 caches: an fp16 copy of v for the prefill kernel, kept by every
 		// append (its P . V products then take P in fp16, one MFMA each); null
@@ -178,6 +179,7 @@ struct nnc_hip_kv
 	int device = 0;
 	int n_cu = 256;
 	bool bf16 = true;
+	bool q4 = false; // a 4-bit cache (bf16 is false)
 	bool exact_batches = false; // batches over kSessionBatch tokens on the split-K path too
 	hipStream_t stream = nullptr;
 	std::vector<kv_buffer> bufs;
@@ -347,6 +349,28 @@ namespace
 		return NNC_OK;
 	}
 
+	// Makes a cache's device current for a call's launches and allocations.
+	class device_scope
+	{
+	public:
+		explicit device_scope(int device) : want_(device)
+		{
+			if (hipGetDevice(&was_) != hipSuccess || was_ == want_) was_ = want_;
+			else (void)hipSetDevice(want_);
+		}
+		~device_scope()
+		{
+			if (was_ != want_) (void)hipSetDevice(was_);
+		}
+		device_scope(const device_scope&) = delete;
+		device_scope& operator=(const device_scope&) = delete;
+
+	private:
+		int want_, was_ = 0;
+	};
+
+	const char* kind_name(const nnc_hip_kv* kv) { return kv->q4 ? "4-bit" : kv->bf16 ? "BF16" : "F32"; }
+
 	nnc_status check_kv(const nnc_hip_kv* kv, int32_t buf)
 	{
 		if (!kv) return fail(NNC_ERR_INVALID_ARGUMENT, "the cache is NULL");
@@ -396,6 +420,37 @@ namespace
 		return NNC_OK;
 	}
 
+	// Host rows in the 4-bit cache's interchange form. A block whose values would
+	// not all be finite is refused: no kernel looks for such values.
+	nnc_status append_raw_q4(nnc_hip_kv* kv, int32_t buf, int32_t pos0, int32_t n_tok, const void* k_rows, const void* v_rows)
+	{
+		const device_scope on(kv->device);
+		const kv_buffer& b = kv->bufs[buf];
+		const size_t blocks = static_cast<size_t>(b.kv_dim / nnchip::kQ4Block), bytes = blocks * n_tok * nnchip::kQ4RawBlock;
+		for (const void* rows : {k_rows, v_rows})
+			for (size_t i = 0; i < blocks * n_tok; ++i)
+			{
+				_Float16 sz[2];
+				std::memcpy(sz, static_cast<const char*>(rows) + i * nnchip::kQ4RawBlock, sizeof sz);
+				const float s = static_cast<float>(sz[0]), z = static_cast<float>(sz[1]);
+				if (!(std::fabs(z) + 15.0f * std::fabs(s) < 65520.0f))
+					return fail(NNC_ERR_INVALID_ARGUMENT, "row %zu, block %zu: scale %g and offset %g stand for values past FP16",
+					            i / blocks, i % blocks, static_cast<double>(s), static_cast<double>(z));
+			}
+		if (nnc_status s = reserve(kv, kv->rows_k, bytes, "append staging")) return s;
+		if (nnc_status s = reserve(kv, kv->rows_v, bytes, "append staging")) return s;
+		if (nnc_status s = reserve_pinned(kv, 2 * bytes, "append staging")) return s;
+		char* pk = static_cast<char*>(kv->pinned.ptr);
+		std::memcpy(pk, k_rows, bytes);
+		std::memcpy(pk + bytes, v_rows, bytes);
+		NNC_HIP_TRY(hipMemcpyAsync(kv->rows_k.ptr, pk, bytes, hipMemcpyHostToDevice, kv->stream), "K/V append");
+		NNC_HIP_TRY(hipMemcpyAsync(kv->rows_v.ptr, pk + bytes, bytes, hipMemcpyHostToDevice, kv->stream), "K/V append");
+		NNC_HIP_TRY(hipEventRecord(kv->pinned.free, kv->stream), "K/V append");
+		nnchip::launch_append_q4(b.k, kv->rows_k.ptr, kv->rows_v.ptr, b.rows, b.kv_dim, pos0, n_tok, true, kv->stream);
+		NNC_HIP_TRY(hipGetLastError(), "K/V append");
+		return NNC_OK;
+	}
+
 	// Shortest split, in wavefront chunks: what one CU keeps in flight
 	// bounds a work-group's loads (about 17 bytes per clock measured with
 	// 128 KiB per CU), so a short span goes to more work-groups with fewer
@@ -423,6 +478,16 @@ namespace
 			sk = (sk + wgk - 1) / wgk * wgk;
 		while ((kmax / sk) - (kmin / sk) + 1 > nnchip::kDecodeMaxSplits) sk += sk < wgk ? unit : wgk;
 		return static_cast<int>(sk);
+	}
+
+	// Keys per work-group of the 4-bit cache's split kernel for one token's span:
+	// about two work-groups per CU (what its registers let be resident up to
+	// head_dim 128), at most kSplitsPerGroupMax per KV head, in whole rounds of a
+	// work-group's wavefronts, or for short spans in units.
+	int split_keys_q4(const nnc_hip_kv* kv, int kmin, int kmax, int n_kv, int head_dim)
+	{
+		return split_keys_for(kv, kmin, kmax, head_dim <= 128 ? (n_kv + 1) / 2 : n_kv, nnchip::kQ4UnitKeys * nnchip::kQ4Waves,
+		                      nnchip::kQ4UnitKeys);
 	}
 
 	// One split-K launch: tokens t0 .. t0 + n - 1 of a call on the absolute
@@ -555,7 +620,8 @@ namespace
 		// One-token launches of the MFMA kernels over a few splits merge in
 		// the split launch; the counts are the cache's, used in stream order.
 		if (nnchip::mfma_shape(head_dim, group) && n_kv <= nnchip::kFuseCounts) p.counts = kv->counts;
-		if (!nnchip::launch_decode(p, n_tok, head_dim, group, kv->bf16, kv->stream))
+		if (kv->q4 ? !nnchip::launch_decode_q4(p, n_tok, head_dim, group, kv->stream)
+		           : !nnchip::launch_decode(p, n_tok, head_dim, group, kv->bf16, kv->stream))
 			return fail(NNC_ERR_UNSUPPORTED_MODEL, "no decode kernel for head_dim %d, group %d", head_dim, group);
 		NNC_HIP_TRY(hipGetLastError(), "decode launch");
 		return NNC_OK;
@@ -569,6 +635,7 @@ namespace
 	void plan_tokens(const nnc_hip_kv* kv, int32_t n_tok, int32_t pos0, int32_t n_seq, int32_t window, bool causal,
 	                 int32_t n_kv, int32_t head_dim, int group, std::vector<decode_plan>& plan)
 	{
+		// (a 4-bit cache has a rule of its own, split_keys_q4)
 		const int wgk = nnchip::decode_wg_keys(head_dim, group, kv->bf16, n_kv);
 		const int unit = nnchip::decode_chunk_keys(head_dim, group, kv->bf16);
 		const int groups = nnchip::decode_groups(n_kv, kv->bf16, head_dim, group);
@@ -578,6 +645,7 @@ namespace
 		{
 			int first, last;
 			span_of(t, first, last);
+			if (kv->q4) return split_keys_q4(kv, first, last, n_kv, head_dim);
 			return split_keys_for(kv, first, last, groups, wgk, unit);
 		};
 		for (int32_t t = 0; t < n_tok;)
@@ -722,6 +790,7 @@ namespace
 	                       int32_t n_seq, int32_t window, bool causal, int32_t n_head, int32_t n_kv, int32_t head_dim,
 	                       float scale, const part_source& src = part_source{})
 	{
+		const device_scope on(kv->device);
 		const kv_buffer& b = kv->bufs[buf];
 		const int group = n_head / n_kv;
 		const bool bf16 = kv->bf16;
@@ -744,7 +813,7 @@ namespace
 		// chunk's span).
 		std::vector<decode_plan> plan;
 		const bool mfma = nnchip::mfma_shape(head_dim, group), tiled = nnchip::tiled_shape_ok(head_dim, group);
-		if (n_tok <= kSessionBatch || kv->exact_batches || (bf16 && !mfma && !tiled))
+		if (n_tok <= kSessionBatch || kv->exact_batches || kv->q4 || (bf16 && !mfma && !tiled))
 			plan_tokens(kv, n_tok, pos0, n_seq, window, causal, n_kv, head_dim, group, plan);
 		else if (bf16 && mfma)
 		{
@@ -824,6 +893,9 @@ namespace
 			            "head_dim %d with group %d is not supported on the GPU (an even head_dim up to 512, group up to "
 			            "%d, group * head_dim up to %d)",
 			            head_dim, group, nnchip::kGenMaxGroup, nnchip::kGenMaxGroupDim);
+		if (kv->q4 && !nnchip::q4_head_dim(head_dim))
+			return fail(NNC_ERR_UNSUPPORTED_MODEL,
+			            "head_dim %d is not supported over a 4-bit cache (32, 64, 96, 128, 192, 256 or 512)", head_dim);
 		if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
 			return fail(NNC_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
 		// The BF16 kernels address a buffer with 32-bit byte offsets.
@@ -864,81 +936,115 @@ namespace
 	}
 }
 
+namespace
+{
+	nnc_status create_cache(int32_t n_buf, const int32_t* rows, const int32_t* kv_dim, bool bf16, bool q4, nnc_hip_kv** out)
+	{
+		if (!out) return fail(NNC_ERR_INVALID_ARGUMENT, "NULL output handle");
+		*out = nullptr;
+		if (n_buf <= 0 || !rows || !kv_dim) return fail(NNC_ERR_INVALID_ARGUMENT, "%d buffers, rows or kv_dim NULL", n_buf);
+		for (int32_t i = 0; i < n_buf; ++i)
+			if (q4 && (rows[i] <= 0 || rows[i] % nnchip::kQ4Rows != 0 || kv_dim[i] <= 0 || kv_dim[i] % nnchip::kQ4Block != 0))
+				return fail(NNC_ERR_INVALID_ARGUMENT, "4-bit buffer %d: %d rows of %d elements (both positive multiples of 32)", i,
+				            rows[i], kv_dim[i]);
+			else if (rows[i] <= 0 || kv_dim[i] <= 0 || kv_dim[i] % 8 != 0)
+				return fail(NNC_ERR_INVALID_ARGUMENT, "buffer %d: %d rows of %d elements (kv_dim must be a positive multiple of 8)",
+				            i, rows[i], kv_dim[i]);
+		int n_dev = 0;
+		if (hipGetDeviceCount(&n_dev) != hipSuccess || n_dev <= 0)
+			return fail(NNC_ERR_UNSUPPORTED_CPU, "no HIP device is available");
+
+		nnc_hip_kv* kv = new (std::nothrow) nnc_hip_kv();
+		if (!kv) return fail(NNC_ERR_OUT_OF_MEMORY, "out of host memory");
+		kv->bf16 = bf16;
+		kv->q4 = q4;
+		auto bail = [&](nnc_status s)
+		{
+			release(kv);
+			return s;
+		};
+		hipError_t e = hipGetDevice(&kv->device);
+		if (e == hipSuccess) e = hipDeviceGetAttribute(&kv->n_cu, hipDeviceAttributeMultiprocessorCount, kv->device);
+		if (e == hipSuccess) e = hipStreamCreateWithFlags(&kv->stream, hipStreamNonBlocking);
+		if (e == hipSuccess) e = hipEventCreateWithFlags(&kv->pinned.free, hipEventDisableTiming);
+		if (e != hipSuccess) return bail(hip_fail(e, "device setup"));
+		const size_t esize = bf16 ? 2 : 4;
+		const bool shadow = bf16 && f16_shadow_enabled();
+		try
+		{
+			kv->bufs.resize(static_cast<size_t>(n_buf));
+		}
+		catch (const std::bad_alloc&)
+		{
+			return bail(fail(NNC_ERR_OUT_OF_MEMORY, "out of host memory"));
+		}
+		if (shadow)
+		{
+			e = hipMalloc(&kv->n_bad, sizeof(int) * static_cast<size_t>(n_buf));
+			if (e == hipSuccess) e = hipMemsetAsync(kv->n_bad, 0, sizeof(int) * static_cast<size_t>(n_buf), kv->stream);
+			if (e != hipSuccess) return bail(hip_fail(e, "K/V allocation"));
+		}
+		for (int32_t i = 0; i < n_buf; ++i)
+		{
+			kv_buffer& b = kv->bufs[i];
+			b.rows = rows[i];
+			b.kv_dim = kv_dim[i];
+			if (q4)
+			{
+				// zeroed: rows never written stand for zeros
+				const size_t bytes = static_cast<size_t>(rows[i] / nnchip::kQ4Rows) * (kv_dim[i] / nnchip::kQ4Block) * nnchip::kQ4Record;
+				e = hipMalloc(&b.k, bytes);
+				if (e == hipSuccess) e = hipMemsetAsync(b.k, 0, bytes, kv->stream);
+				if (e != hipSuccess) return bail(hip_fail(e, "K/V allocation"));
+				kv->bytes += bytes;
+				continue;
+			}
+			const size_t n = static_cast<size_t>(rows[i]) * kv_dim[i] * esize;
+			e = hipMalloc(&b.k, n);
+			if (e == hipSuccess) e = hipMalloc(&b.v_alloc, n + kVOffset);
+			if (e == hipSuccess) b.v = static_cast<char*>(b.v_alloc) + kVOffset;
+			if (e == hipSuccess) e = hipMemsetAsync(b.k, 0, n, kv->stream);
+			if (e == hipSuccess) e = hipMemsetAsync(b.v, 0, n, kv->stream);
+			if (shadow)
+			{
+				// zeroed: rows never written hold finite values, which the prefill
+				// kernels may read (and weigh 0) beside a group's written rows
+				const size_t n16 = nnchip::f16_copy_bytes(rows[i], kv_dim[i]);
+				if (e == hipSuccess) e = hipMalloc(&b.v16_alloc, n16 + kVOffset);
+				if (e == hipSuccess) b.v16 = static_cast<char*>(b.v16_alloc) + kVOffset;
+				if (e == hipSuccess) e = hipMemsetAsync(b.v16, 0, n16, kv->stream);
+				kv->bytes += n16;
+			}
+			if (e != hipSuccess) return bail(hip_fail(e, "K/V allocation"));
+			kv->bytes += 2 * n;
+		}
+		e = hipMalloc(&kv->counts, sizeof(unsigned) * nnchip::kFuseCounts);
+		if (e == hipSuccess) e = hipMemsetAsync(kv->counts, 0, sizeof(unsigned) * nnchip::kFuseCounts, kv->stream);
+		if (e == hipSuccess) e = hipStreamSynchronize(kv->stream);
+		if (e != hipSuccess) return bail(hip_fail(e, "K/V allocation"));
+		void* fixed = nullptr;
+		if (nnc_status s = noalloc_scratch(kv->device, &fixed)) return bail(s);
+		// The counterpart of nnc's context line (reference session.cpp:341-343).
+		hipDeviceProp_t prop;
+		const bool named = hipGetDeviceProperties(&prop, kv->device) == hipSuccess;
+		log_msg(NNC_HIP_LOG_INFO, "device %d (%s, %d CUs): %d K/V buffers, %.1f MB of %s K/V%s in device memory",
+		        kv->device, named ? prop.name : "unknown", kv->n_cu, n_buf, static_cast<double>(kv->bytes) / 1e6,
+		        kind_name(kv), shadow ? " (with V's fp16 copy)" : "");
+		*out = kv;
+		return NNC_OK;
+	}
+}
+
 extern "C" {
 
 nnc_status nnc_hip_kv_create(int32_t n_buf, const int32_t* rows, const int32_t* kv_dim, bool bf16, nnc_hip_kv** out)
 {
-	if (!out) return fail(NNC_ERR_INVALID_ARGUMENT, "NULL output handle");
-	*out = nullptr;
-	if (n_buf <= 0 || !rows || !kv_dim) return fail(NNC_ERR_INVALID_ARGUMENT, "%d buffers, rows or kv_dim NULL", n_buf);
-	for (int32_t i = 0; i < n_buf; ++i)
-		if (rows[i] <= 0 || kv_dim[i] <= 0 || kv_dim[i] % 8 != 0)
-			return fail(NNC_ERR_INVALID_ARGUMENT, "buffer %d: %d rows of %d elements (kv_dim must be a positive multiple of 8)",
-			            i, rows[i], kv_dim[i]);
-	int n_dev = 0;
-	if (hipGetDeviceCount(&n_dev) != hipSuccess || n_dev <= 0)
-		return fail(NNC_ERR_UNSUPPORTED_CPU, "no HIP device is available");
+	return create_cache(n_buf, rows, kv_dim, bf16, false, out);
+}
 
-	nnc_hip_kv* kv = new (std::nothrow) nnc_hip_kv();
-	if (!kv) return fail(NNC_ERR_OUT_OF_MEMORY, "out of host memory");
-	kv->bf16 = bf16;
-	auto bail = [&](nnc_status s)
-	{
-		release(kv);
-		return s;
-	};
-	hipError_t e = hipGetDevice(&kv->device);
-	if (e == hipSuccess) e = hipDeviceGetAttribute(&kv->n_cu, hipDeviceAttributeMultiprocessorCount, kv->device);
-	if (e == hipSuccess) e = hipStreamCreateWithFlags(&kv->stream, hipStreamNonBlocking);
-	if (e == hipSuccess) e = hipEventCreateWithFlags(&kv->pinned.free, hipEventDisableTiming);
-	if (e != hipSuccess) return bail(hip_fail(e, "device setup"));
-	const size_t esize = bf16 ? 2 : 4;
-	const bool shadow = bf16 && f16_shadow_enabled();
-	kv->bufs.resize(static_cast<size_t>(n_buf));
-	if (shadow)
-	{
-		e = hipMalloc(&kv->n_bad, sizeof(int) * static_cast<size_t>(n_buf));
-		if (e == hipSuccess) e = hipMemsetAsync(kv->n_bad, 0, sizeof(int) * static_cast<size_t>(n_buf), kv->stream);
-		if (e != hipSuccess) return bail(hip_fail(e, "K/V allocation"));
-	}
-	for (int32_t i = 0; i < n_buf; ++i)
-	{
-		kv_buffer& b = kv->bufs[i];
-		b.rows = rows[i];
-		b.kv_dim = kv_dim[i];
-		const size_t n = static_cast<size_t>(rows[i]) * kv_dim[i] * esize;
-		e = hipMalloc(&b.k, n);
-		if (e == hipSuccess) e = hipMalloc(&b.v_alloc, n + kVOffset);
-		if (e == hipSuccess) b.v = static_cast<char*>(b.v_alloc) + kVOffset;
-		if (e == hipSuccess) e = hipMemsetAsync(b.k, 0, n, kv->stream);
-		if (e == hipSuccess) e = hipMemsetAsync(b.v, 0, n, kv->stream);
-		if (shadow)
-		{
-			// zeroed: rows never written hold finite values, which the prefill
-			// kernels may read (and weigh 0) beside a group's written rows
-			const size_t n16 = nnchip::f16_copy_bytes(rows[i], kv_dim[i]);
-			if (e == hipSuccess) e = hipMalloc(&b.v16_alloc, n16 + kVOffset);
-			if (e == hipSuccess) b.v16 = static_cast<char*>(b.v16_alloc) + kVOffset;
-			if (e == hipSuccess) e = hipMemsetAsync(b.v16, 0, n16, kv->stream);
-			kv->bytes += n16;
-		}
-		if (e != hipSuccess) return bail(hip_fail(e, "K/V allocation"));
-		kv->bytes += 2 * n;
-	}
-	e = hipMalloc(&kv->counts, sizeof(unsigned) * nnchip::kFuseCounts);
-	if (e == hipSuccess) e = hipMemsetAsync(kv->counts, 0, sizeof(unsigned) * nnchip::kFuseCounts, kv->stream);
-	if (e == hipSuccess) e = hipStreamSynchronize(kv->stream);
-	if (e != hipSuccess) return bail(hip_fail(e, "K/V allocation"));
-	void* fixed = nullptr;
-	if (nnc_status s = noalloc_scratch(kv->device, &fixed)) return bail(s);
-	// The counterpart of nnc's context line (reference session.cpp:341-343).
-	hipDeviceProp_t prop;
-	const bool named = hipGetDeviceProperties(&prop, kv->device) == hipSuccess;
-	log_msg(NNC_HIP_LOG_INFO, "device %d (%s, %d CUs): %d K/V buffers, %.1f MB of %s K/V%s in device memory",
-	        kv->device, named ? prop.name : "unknown", kv->n_cu, n_buf, static_cast<double>(kv->bytes) / 1e6,
-	        bf16 ? "BF16" : "F32", shadow ? " (with V's fp16 copy)" : "");
-	*out = kv;
-	return NNC_OK;
+nnc_status nnc_hip_kv_create_q4(int32_t n_buf, const int32_t* rows, const int32_t* kv_dim, nnc_hip_kv** out)
+{
+	return create_cache(n_buf, rows, kv_dim, false, true, out);
 }
 
 void nnc_hip_kv_free(nnc_hip_kv* kv) { release(kv); }
@@ -963,6 +1069,7 @@ nnc_status nnc_hip_kv_append(nnc_hip_kv* kv, int32_t buf, int32_t pos0, int32_t 
                              const void* v_rows)
 {
 	if (nnc_status s = check_append(kv, buf, pos0, n_tok, k_rows, v_rows)) return s;
+	if (kv->q4) return append_raw_q4(kv, buf, pos0, n_tok, k_rows, v_rows);
 	// Through the pinned staging, straight into the buffer's rows, so the
 	// host rows are free on return.
 	const size_t bytes = static_cast<size_t>(n_tok) * kv->bufs[buf].kv_dim * (kv->bf16 ? 2 : 4);
@@ -997,7 +1104,16 @@ nnc_status nnc_hip_kv_append_f32_device(nnc_hip_kv* kv, int32_t buf, int32_t pos
                                         const float* v_rows)
 {
 	if (nnc_status s = check_append(kv, buf, pos0, n_tok, k_rows, v_rows)) return s;
+	const device_scope on(kv->device);
 	const kv_buffer& b = kv->bufs[buf];
+	if (kv->q4)
+	{
+		if ((reinterpret_cast<uintptr_t>(k_rows) | reinterpret_cast<uintptr_t>(v_rows)) & 15)
+			return fail(NNC_ERR_INVALID_ARGUMENT, "rows for a 4-bit cache must be 16-byte aligned");
+		nnchip::launch_append_q4(b.k, k_rows, v_rows, b.rows, b.kv_dim, pos0, n_tok, false, kv->stream);
+		NNC_HIP_TRY(hipGetLastError(), "K/V append");
+		return NNC_OK;
+	}
 	nnchip::launch_append_f32(b.k, b.v, k_rows, v_rows, b.rows, b.kv_dim, pos0, n_tok, kv->bf16, kv->stream, b.v16,
 	                          b.v16 ? kv->n_bad + buf : nullptr);
 	NNC_HIP_TRY(hipGetLastError(), "K/V append");
@@ -1048,10 +1164,23 @@ nnc_status nnc_hip_kv_prep_append_device(nnc_hip_kv* kv, int32_t buf, int32_t po
 	p.eps = pr.rms_eps;
 	p.inv_dim = 1.0f / static_cast<float>(pr.head_dim); // (reference nn_ops.cpp:594)
 	p.rope_cs = nullptr;
+	const device_scope on(kv->device);
+	if (kv->q4)
+	{
+		// K and V normalised and rotated into F32 rows 0 .. n_tok - 1, quantised from there
+		const size_t bytes = static_cast<size_t>(n_tok) * b.kv_dim * sizeof(float);
+		if (nnc_status s = reserve(kv, kv->rows_k, bytes, "pre-attention rows")) return s;
+		if (nnc_status s = reserve(kv, kv->rows_v, bytes, "pre-attention rows")) return s;
+		p.K = kv->rows_k.ptr;
+		p.V = kv->rows_v.ptr;
+		p.rows = n_tok;
+		p.pos0 = 0;
+	}
 	if (pr.n_rot > 0)
 		if (nnc_status s = rope_cs(kv, pr, pos0, n_tok, p.rope_cs)) return s;
 	if (!nnchip::launch_prep(p, n_tok, kv->stream))
 		return fail(NNC_ERR_UNSUPPORTED_MODEL, "no pre-attention kernel for head_dim %d", pr.head_dim);
+	if (kv->q4) nnchip::launch_append_q4(b.k, p.K, p.V, b.rows, b.kv_dim, pos0, n_tok, false, kv->stream);
 	NNC_HIP_TRY(hipGetLastError(), "pre-attention step");
 	return NNC_OK;
 }
@@ -1062,6 +1191,22 @@ nnc_status nnc_hip_kv_read(nnc_hip_kv* kv, int32_t buf, int32_t row0, int32_t n_
 	const kv_buffer& b = kv->bufs[buf];
 	if (row0 < 0 || n_rows < 0 || row0 + static_cast<long long>(n_rows) > b.rows)
 		return fail(NNC_ERR_INVALID_ARGUMENT, "rows %d .. %d outside a buffer of %d", row0, row0 + n_rows - 1, b.rows);
+	if (kv->q4)
+	{
+		// through device rows in the interchange form
+		const device_scope on(kv->device);
+		const size_t bytes = static_cast<size_t>(n_rows) * (b.kv_dim / nnchip::kQ4Block) * nnchip::kQ4RawBlock;
+		if (n_rows == 0 || (!k_out && !v_out)) return nnc_hip_kv_sync(kv);
+		if (nnc_status s = reserve(kv, kv->rows_k, bytes, "K/V read")) return s;
+		if (nnc_status s = reserve(kv, kv->rows_v, bytes, "K/V read")) return s;
+		nnchip::launch_read_q4(b.k, k_out ? kv->rows_k.ptr : nullptr, v_out ? kv->rows_v.ptr : nullptr, b.kv_dim, row0, n_rows,
+		                       true, kv->stream);
+		NNC_HIP_TRY(hipGetLastError(), "K/V read");
+		if (k_out) NNC_HIP_TRY(hipMemcpyAsync(k_out, kv->rows_k.ptr, bytes, hipMemcpyDeviceToHost, kv->stream), "K/V read");
+		if (v_out) NNC_HIP_TRY(hipMemcpyAsync(v_out, kv->rows_v.ptr, bytes, hipMemcpyDeviceToHost, kv->stream), "K/V read");
+		NNC_HIP_TRY(hipStreamSynchronize(kv->stream), "K/V read");
+		return NNC_OK;
+	}
 	const size_t row_bytes = static_cast<size_t>(b.kv_dim) * (kv->bf16 ? 2 : 4);
 	const size_t off = static_cast<size_t>(row0) * row_bytes, n = static_cast<size_t>(n_rows) * row_bytes;
 	if (k_out && n)
@@ -1069,6 +1214,25 @@ nnc_status nnc_hip_kv_read(nnc_hip_kv* kv, int32_t buf, int32_t row0, int32_t n_
 	if (v_out && n)
 		NNC_HIP_TRY(hipMemcpyAsync(v_out, static_cast<char*>(b.v) + off, n, hipMemcpyDeviceToHost, kv->stream), "K/V read");
 	NNC_HIP_TRY(hipStreamSynchronize(kv->stream), "K/V read");
+	return NNC_OK;
+}
+
+nnc_status nnc_hip_kv_read_f32_device(nnc_hip_kv* kv, int32_t buf, int32_t row0, int32_t n_rows, float* k_out, float* v_out)
+{
+	if (nnc_status s = check_kv(kv, buf)) return s;
+	const kv_buffer& b = kv->bufs[buf];
+	if (row0 < 0 || n_rows < 0 || row0 + static_cast<long long>(n_rows) > b.rows)
+		return fail(NNC_ERR_INVALID_ARGUMENT, "%d rows from %d on outside a buffer of %d", n_rows, row0, b.rows);
+	if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15)
+		return fail(NNC_ERR_INVALID_ARGUMENT, "outputs must be 16-byte aligned");
+	if (n_rows == 0 || (!k_out && !v_out)) return NNC_OK;
+	const device_scope on(kv->device);
+	if (kv->q4)
+		nnchip::launch_read_q4(b.k, k_out, v_out, b.kv_dim, row0, n_rows, false, kv->stream);
+	else
+		nnchip::launch_read_rows(b.k, b.v, k_out, v_out, static_cast<size_t>(row0) * b.kv_dim,
+		                         static_cast<size_t>(n_rows) * b.kv_dim, kv->bf16, kv->stream);
+	NNC_HIP_TRY(hipGetLastError(), "K/V read");
 	return NNC_OK;
 }
 

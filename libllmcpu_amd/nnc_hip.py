@@ -122,6 +122,7 @@ LOG_CALLBACK = C.CFUNCTYPE(None, C.c_int, C.c_char_p, C.c_void_p)
 SIGNATURES = {
     "nnc_hip_set_log_callback": (None, [LOG_CALLBACK, _P]),
     "nnc_hip_kv_create": (C.c_int, [_I, C.POINTER(_I), C.POINTER(_I), _B, C.POINTER(_P)]),
+    "nnc_hip_kv_create_q4": (C.c_int, [_I, C.POINTER(_I), C.POINTER(_I), C.POINTER(_P)]),
     "nnc_hip_kv_free": (None, [_P]),
     "nnc_hip_kv_bytes": (_U64, [_P]),
     "nnc_hip_kv_set_exact_batches": (C.c_int, [_P, _B]),
@@ -130,6 +131,7 @@ SIGNATURES = {
     "nnc_hip_kv_append_f32_device": (C.c_int, [_P, _I, _I, _I, _P, _P]),
     "nnc_hip_kv_prep_append_device": (C.c_int, [_P, _I, _I, _I, _P, _P, _P, C.POINTER(NncHipPrep)]),
     "nnc_hip_kv_read": (C.c_int, [_P, _I, _I, _I, _P, _P]),
+    "nnc_hip_kv_read_f32_device": (C.c_int, [_P, _I, _I, _I, _P, _P]),
     "nnc_hip_attend": (C.c_int, [_P, _I, _P, _P, _I, _I, _I, _I, _B, _I, _I, _I, _F]),
     "nnc_hip_attend_device": (C.c_int, [_P, _I, _P, _P, _I, _I, _I, _I, _B, _I, _I, _I, _F]),
     "nnc_hip_attend_device_noalloc": (C.c_int, [_P, _I, _P, _P, _I, _I, _I, _I, _B, _I, _I, _I, _F]),
@@ -243,9 +245,10 @@ def bf16_to_f32(b: np.ndarray) -> np.ndarray:
 
 class KVCache:
     """A session's K/V buffers in HBM. `rows[i]` and `kv_dim[i]` size buffer i
-    as model_kv_init would; `bf16` picks the element type (nnc_kv_type)."""
+    as model_kv_init would; `bf16` picks the element type (nnc_kv_type), `q4`
+    the 4-bit cache (rows and kv_dim multiples of 32)."""
 
-    def __init__(self, rows: list[int], kv_dim: list[int], bf16: bool = True):
+    def __init__(self, rows: list[int], kv_dim: list[int], bf16: bool = True, *, q4: bool = False):
         lib = load_library()
         n = len(rows)
         if len(kv_dim) != n:
@@ -253,12 +256,16 @@ class KVCache:
         r = (_I * n)(*rows)
         d = (_I * n)(*kv_dim)
         h = _P()
-        _check(lib.nnc_hip_kv_create(n, r, d, bool(bf16), C.byref(h)))
+        if q4:
+            _check(lib.nnc_hip_kv_create_q4(n, r, d, C.byref(h)))
+        else:
+            _check(lib.nnc_hip_kv_create(n, r, d, bool(bf16), C.byref(h)))
         self._lib = lib
         self.handle = h
         self.rows = list(rows)
         self.kv_dim = list(kv_dim)
-        self.bf16 = bool(bf16)
+        self.bf16 = bool(bf16) and not q4
+        self.q4 = bool(q4)
 
     def close(self) -> None:
         if self.handle:
@@ -290,30 +297,63 @@ class KVCache:
         bits of its one-token call (default False: the prefill kernel)."""
         _check(self._lib.nnc_hip_kv_set_exact_batches(self.handle, bool(exact)))
 
+    def _row(self, buf: int) -> tuple[type, int]:
+        """Element type and elements of a row in the cache's own form: uint16 BF16
+        bits, float32, or the 4-bit blocks' bytes (s and z in FP16, 16 of codes)."""
+        d = self.kv_dim[buf] if 0 <= buf < len(self.kv_dim) else 0
+        return (np.uint8, d // 32 * 20) if self.q4 else (np.uint16 if self.bf16 else np.float32, d)
+
     def append(self, buf: int, pos0: int, k: np.ndarray, v: np.ndarray) -> None:
-        """Rows already in the cache's element type: uint16 BF16 bits, or float32."""
-        dt = np.uint16 if self.bf16 else np.float32
+        """Rows already in the cache's element type: uint16 BF16 bits, float32, or
+        uint8 rows of 4-bit blocks."""
+        dt, d = self._row(buf)
         k = np.ascontiguousarray(k, dtype=dt)
         v = np.ascontiguousarray(v, dtype=dt)
-        n_tok = k.size // self.kv_dim[buf] if 0 <= buf < len(self.kv_dim) else 0
+        n_tok = k.size // d if d else 0
         _check(self._lib.nnc_hip_kv_append(self.handle, buf, pos0, n_tok, _ptr(k), _ptr(v)))
         self.sync()
 
     def append_f32(self, buf: int, pos0: int, k: np.ndarray, v: np.ndarray) -> None:
-        """F32 rows; a BF16 cache rounds them on the device (nnc_f32_to_bf16 bits)."""
+        """F32 rows; a BF16 cache rounds them on the device (nnc_f32_to_bf16 bits),
+        a 4-bit one quantises them there."""
         k = np.ascontiguousarray(k, dtype=np.float32)
         v = np.ascontiguousarray(v, dtype=np.float32)
         n_tok = k.size // self.kv_dim[buf] if 0 <= buf < len(self.kv_dim) else 0
         _check(self._lib.nnc_hip_kv_append_f32(self.handle, buf, pos0, n_tok, _ptr(k), _ptr(v)))
         self.sync()
 
+    def append_f32_device(self, buf: int, k_dev: int, v_dev: int, *, pos0: int, n_tok: int) -> None:
+        """append_f32 from device addresses; queued on the cache's stream."""
+        _check(self._lib.nnc_hip_kv_append_f32_device(self.handle, buf, pos0, n_tok, k_dev, v_dev))
+
     def read(self, buf: int, row0: int, n_rows: int) -> tuple[np.ndarray, np.ndarray]:
-        dt = np.uint16 if self.bf16 else np.float32
-        d = self.kv_dim[buf]
+        dt, d = self._row(buf)
         k = np.empty((n_rows, d), dtype=dt)
         v = np.empty((n_rows, d), dtype=dt)
         _check(self._lib.nnc_hip_kv_read(self.handle, buf, row0, n_rows, _ptr(k), _ptr(v)))
         return k, v
+
+    def read_f32_device(self, buf: int, row0: int, n_rows: int, k_dev: int, v_dev: int) -> None:
+        """The values of rows row0 .. row0 + n_rows - 1 as float32 rows at device
+        addresses (0: not that one); queued on the cache's stream."""
+        _check(self._lib.nnc_hip_kv_read_f32_device(self.handle, buf, row0, n_rows, k_dev or None, v_dev or None))
+
+    def read_f32(self, buf: int, row0: int, n_rows: int) -> tuple[np.ndarray, np.ndarray]:
+        """read_f32_device to host arrays (through scratch device memory, freed afterwards)."""
+        from . import hip_rt
+
+        d = self.kv_dim[buf] if 0 <= buf < len(self.kv_dim) else 0
+        k, v = np.empty((max(n_rows, 0), d), np.float32), np.empty((max(n_rows, 0), d), np.float32)
+        dev = []
+        try:
+            for a in (k, v):
+                dev.append(hip_rt.malloc(max(a.nbytes, 16)))
+            self.read_f32_device(buf, row0, n_rows, *dev)
+            self.sync()
+            return hip_rt.to_host(k, dev[0]), hip_rt.to_host(v, dev[1])
+        finally:
+            for p in dev:
+                hip_rt.free(p)
 
     def attend(self, buf: int, q: np.ndarray, *, pos0: int, n_seq: int | None = None, window: int = 0,
                causal: bool = True, n_head: int, n_kv: int, head_dim: int, scale: float,

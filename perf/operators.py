@@ -15,7 +15,8 @@ elementary torch operations:
 A cache's block is 32 consecutive elements of a row: with lo and hi its least
 and largest element, s = f16((hi - lo) / 15), z = f16(lo), an element x is the
 whole number c = rint((x - z) / s) within 0 .. 15 (0 where s is 0) and stands
-for f16(c s + z), rounded once.
+for f16(c s + z), rounded once. (Elements are first brought within +-65280, so
+that no value overflows f16.)
 
 Head shapes are those of the models this repository's benchmark and tests
 name, and a few others. Cached keys have the per-channel offsets that make a
@@ -125,7 +126,7 @@ def _kv_rows(seed, n, kv_dim, head_dim):
 
 def _quantised(x):
     """(codes, two to a byte: elements i and i + 16 of a block in byte i; scale; offset) of F32 rows."""
-    b = x.clamp(-65504.0, 65504.0).view(x.shape[0], -1, 32)
+    b = x.clamp(-65280.0, 65280.0).view(x.shape[0], -1, 32)
     lo, hi = b.amin(-1), b.amax(-1)
     s, z = ((hi - lo) / 15.0).half(), lo.half()
     c = torch.where(s[..., None] > 0, torch.round((b - z.float()[..., None]) / s.float()[..., None]), torch.zeros_like(b))
