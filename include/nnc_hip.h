@@ -104,8 +104,8 @@ nnc_status nnc_hip_kv_create(int32_t n_buf, const int32_t* rows, const int32_t* 
  * and F32. A block is 32 consecutive elements of a row, nnc's own 4-bit weight
  * block (reference nn_ops.h:138-142) along the head: with lo and hi its least
  * and largest element,
- *   s = f16((hi - lo) / 15), z = f16(lo), c = rint((x - z) / s) in 0 .. 15
- * (0 where s is 0), and x is held as f16(c * s + z), rounded once. Elements
+ *   s = f16((hi - lo) * r), z = f16(lo), c = rint((x - z) / s) in 0 .. 15
+ * (0 where s is 0; r is 1 / 15 in F32, all of it in F32), and x is held as f16(c * s + z), rounded once. Elements
  * are brought within +-65280 first and a NaN is held as 0, so every value of
  * such a cache is finite. The other calls take it as they take the others:
  *   nnc_hip_kv_append_f32, _f32_device and nnc_hip_kv_prep_append_device

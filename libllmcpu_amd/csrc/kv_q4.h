@@ -4,7 +4,7 @@
 // Format. A block is 32 consecutive elements of a row (nnc's own 4-bit block,
 // reference nn_ops.h:138-142, along the head instead of a weight row). With lo
 // and hi its least and largest element,
-//   s = f16((hi - lo) / 15),  z = f16(lo),
+//   s = f16((hi - lo) r), r = 1 / 15 in fp32,  z = f16(lo),
 //   c = rint((x - z) / s) within 0 .. 15 (0 where s is 0),
 // and the element stands for f16(c s + z), rounded once: one fused multiply-add
 // in fp16, which is what the attention kernels feed to the matrix cores, so

@@ -13,7 +13,7 @@ def quantise(x: np.ndarray):
     x = np.where(np.isnan(x), np.float32(0), x).astype(np.float32)
     b = np.clip(x, np.float32(-Q4_MAX), np.float32(Q4_MAX)).reshape(x.shape[0], -1, 32)
     lo, hi = b.min(-1), b.max(-1)
-    s, z = ((hi - lo) / np.float32(15)).astype(np.float16), lo.astype(np.float16)
+    s, z = ((hi - lo) * (np.float32(1) / np.float32(15))).astype(np.float16), lo.astype(np.float16)
     sf, zf = s.astype(np.float32)[..., None], z.astype(np.float32)[..., None]
     with np.errstate(divide="ignore", invalid="ignore"):
         c = np.where(sf > 0, np.rint((b - zf) / sf), 0)
