@@ -301,6 +301,43 @@ nnc_status nnc_hip_attend_gated_device(nnc_hip_kv* kv, int32_t buf, const float*
                                        int32_t n_tok, int32_t pos0, int32_t n_seq, int32_t window, bool causal,
                                        int32_t n_head, int32_t n_kv, int32_t head_dim, float scale);
 
+/* Element types of nnc_hip_attend_packed_device. */
+enum
+{
+	NNC_HIP_F32 = 0,
+	NNC_HIP_BF16 = 1
+};
+
+/* Attention over several whole sequences laid end to end, without a cache: the
+ * prompts of several requests, or the texts of an embedding batch (nnc's
+ * embedding call takes one text, reference model.cpp:2344-2384; no counterpart
+ * in nnc). Sequence s has rows starts[s] .. starts[s + 1] - 1 of q, k, v and
+ * out; its first row is position 0, and row i of it attends to the keys of
+ * model_attn_span(causal, window, i, its length): its own sequence alone, so
+ * each gets what nnc_hip_attend gives for it by itself over a cache of those
+ * rows.
+ *   starts: host memory, n_seqs + 1 row numbers, not decreasing, read before
+ *     the call returns; empty sequences are allowed, and rows before the first
+ *     start and from the last one on are neither read nor written;
+ *   q, out [rows][n_head * head_dim], k, v [rows][n_kv * head_dim]: device
+ *     memory, elements of `type` (NNC_HIP_F32 or NNC_HIP_BF16 bit patterns),
+ *     rows *_stride elements apart, so the four may be columns of one buffer;
+ *     out may be q.
+ * head_dim a multiple of 8 up to 256, any group n_head / n_kv. F32: the error
+ * of fp32 sums; BF16: weights rounded to BF16, sums in fp32, rounded once to
+ * out. An infinite or NaN element of a key reaches only the rows that attend
+ * it. `kv` is the execution context; queued on its stream, nothing is
+ * allocated, and the call may be captured (the starts are then the graph's).
+ * NNC_ERR_INVALID_ARGUMENT: NULL pointers, an unknown type, starts that
+ * decrease or are negative, n_head not a multiple of n_kv, pointers not
+ * 16-byte aligned, strides below the row, not whole 16 bytes, or of 2^23
+ * elements and more.
+ * NNC_ERR_UNSUPPORTED_MODEL: another head_dim. */
+nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void* q, size_t q_stride, const void* k,
+                                        size_t k_stride, const void* v, size_t v_stride, void* out, size_t out_stride,
+                                        const int32_t* starts, int32_t n_seqs, int32_t window, bool causal, int32_t n_head,
+                                        int32_t n_kv, int32_t head_dim, float scale);
+
 /* The weight gemvs on either side of attention (QKV and output projections,
  * MLP, lm_head; reference model.cpp:1189-1210 picks one by tensor type):
  *   Y[n][r] = sum_k W[r][k] * X[n][k],  n < n_batch, r < rows, k < cols,

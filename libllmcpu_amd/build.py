@@ -17,7 +17,7 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libnnc_hip.so"
 SOURCES = ["nnc_hip.hip", "attn_decode.hip", "attn_generic.hip", "attn_tiled.hip", "attn_prefill.hip", "attn_q4.hip",
-           "kv_ops.hip", "kv_prep.hip", "kv_q4.hip", "gemv.hip"]
+           "attn_flash.hip", "kv_ops.hip", "kv_prep.hip", "kv_q4.hip", "gemv.hip"]
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CFLAGS = [

@@ -1,0 +1,701 @@
+// Attention of many query rows over whole sequences on the matrix cores: packed
+// prompts (BF16 or F32 q, k, v in device memory, several sequences end to end)
+// and batches over the 4-bit cache (kv_q4.h).
+//
+// The rows of a KV head are (token, query head) pairs, token by token, so the
+// heads that share its keys share every load. A work-group of four wavefronts
+// owns 128 rows of one sequence and walks their keys in steps: the step's K, and
+// V transposed, go to LDS once for all rows, and each wavefront computes for its
+// 32 rows
+//   S^T = K Q^T        (a lane holds 16 keys' scores of one row per 32 x 32 tile)
+//   P = 2^(S - offset) (running offset and sum per row; see kRaise)
+//   O^T += V^T P^T     (the lane's own weights are the operand: a lane's eight k
+//                       slots of a product are taken to be the keys it holds)
+// One pass over the keys; only steps that cross a row's span are masked.
+//
+// Precision. BF16: the operands are exact, P is rounded to BF16 (2^-9 of a
+// weight; the output is rounded to BF16 as well). F32 and the 4-bit cache, whose
+// outputs are F32: Q, P and F32's K and V are fp16 hi + lo (22 bits), brought
+// into fp16's range by powers of two (per row of Q, per step for K, running for
+// V), the product of two lo parts left out: 3 products for F32, 2 over the 4-bit
+// cache, whose values are fp16 themselves. Scores, sums and outputs are fp32.
+//
+// Elements that are infinite or NaN: a key's reach only the rows that attend it.
+// Scores of masked keys are replaced, but 0 x inf in P V is not, and inf has no
+// lo part: a work-group that meets such an element in a masked step (F32: in any
+// step) computes its rows anew in fp32 on the vector ALUs, each over its own
+// span.
+#include "kernels.h"
+#include "kv_q4.h"
+
+#include <type_traits>
+
+namespace nnchip
+{
+	namespace
+	{
+		constexpr int kBf16 = 0, kF32 = 1, kQ4 = 2;
+		constexpr int kWaves = 4, kRows = 32 * kWaves;
+		// Weights are 2^(score - offset); the offset is raised, to kBelow under the
+		// largest score so far, when a score passes it by more than kRaise: weights
+		// stay in fp16's range, and rescaling O is rare.
+		constexpr float kRaise = 14.0f, kBelow = 6.0f;
+
+		constexpr int kBufferFlags = 0x00020000; // buffer descriptor word 3: raw 32-bit data
+
+		template <int MODE, int HD>
+		struct shape
+		{
+			static constexpr int KS = HD <= 128 ? 64 : 32; // keys of a step
+			static constexpr int KT = KS / 32; // 32-key tiles
+			static constexpr int KP = HD + 8, VP = KS + 8; // halves per K row, per V^T row (an odd number of 16 bytes)
+			static constexpr int PARTS = MODE == kF32 ? 2 : 1; // hi, lo
+			static constexpr int K_HALVES = KS * KP, V_HALVES = HD * VP;
+			static constexpr int TILE_BYTES = 2 * PARTS * (K_HALVES + V_HALVES);
+			static constexpr int BYTES = TILE_BYTES;
+			static constexpr int NK = KS * HD / 8 / 256; // 8-element pieces of K per thread
+			static constexpr int NV = (HD / 2 * (KS / 8) + 255) / 256; // (column pair, 8 keys) pieces of V per thread
+			static constexpr int NR = (KS / 32 * (HD / 32) + kWaves - 1) / kWaves; // records per wavefront
+			static constexpr int PER_SIMD = HD <= (MODE == kBf16 ? 128 : 64) ? 2 : 1; // wavefronts
+		};
+
+		// What a step's loads leave in registers until LDS is free.
+		template <int MODE, int HD>
+		struct step_regs
+		{
+			u32x4 k[shape<MODE, HD>::NK * shape<MODE, HD>::PARTS];
+			uint32_t v[shape<MODE, HD>::NV][8 * shape<MODE, HD>::PARTS];
+		};
+		// (4-bit: the wavefront's records)
+		template <int HD>
+		struct step_regs<kQ4, HD>
+		{
+			u32x4 code[shape<kQ4, HD>::NR];
+			u32x2 ksz[shape<kQ4, HD>::NR];
+			u32x4 vs[shape<kQ4, HD>::NR], vz[shape<kQ4, HD>::NR];
+		};
+
+		__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+		// The largest of x over the wavefront.
+		__device__ __forceinline__ uint32_t wave_umax(uint32_t x)
+		{
+			x = umax(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xf, 0xf, false));
+			x = umax(x, __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xf, 0xf, false));
+			x = umax(x, __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false));
+			x = umax(x, __builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, false));
+			const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+			x = umax(r[0], r[1]);
+			const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+			return umax(s[0], s[1]);
+		}
+
+		// The power of two that brings a largest magnitude (its bits) under 2^15; 0
+		// for zero.
+		__device__ __forceinline__ int up_to_2_15(uint32_t bits)
+		{
+			return bits == 0 ? 0 : 14 - ilogbf(__uint_as_float(bits));
+		}
+
+		// Two values as fp16 hi and lo pairs, both rounded to nearest: a lo part is
+		// at most 2^-11 of its value and of either sign, so leaving out the products
+		// of two lo parts (2^-22 at most) adds no bias.
+		__device__ __forceinline__ void split_f16x2(float a, float b, uint32_t& hi, uint32_t& lo)
+		{
+			const f16x2 h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+			hi = as_u32(h);
+			lo = pack_f16x2(a - static_cast<float>(h.x), b - static_cast<float>(h.y));
+		}
+		// The same for weights, hi cut instead of rounded (one instruction for both):
+		// their lo parts meet V's lo parts only, which have either sign.
+		__device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& lo)
+		{
+			const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+			hi = __builtin_bit_cast(uint32_t, h);
+			lo = pack_f16x2(a - static_cast<float>(h[0]), b - static_cast<float>(h[1]));
+		}
+
+		// A row's attention in fp32 on the vector ALUs by one wavefront, every
+		// operand straight from memory: 64 keys at a time, a lane per key for the
+		// scores and per column for the outputs.
+		template <int MODE>
+		__device__ void vector_row(const flash_params& p, size_t row_at, int tok, int head, int kvh, int first, int last, int lane)
+		{
+			auto el = [](const void* b, size_t i)
+			{
+				if constexpr (MODE == kBf16) return bf16_bits_to_f32(static_cast<const uint16_t*>(b)[i]);
+				else return static_cast<const float*>(b)[i];
+			};
+			const int hd = p.head_dim;
+			const size_t qi = (row_at + tok) * p.q_stride + static_cast<size_t>(head) * hd, col = static_cast<size_t>(kvh) * hd;
+			float o[kFlashMaxDim / 64] = {};
+			float m = -INFINITY, l = 0.0f;
+			for (int k0 = first; k0 <= last; k0 += 64)
+			{
+				float s = -INFINITY;
+				if (k0 + lane <= last)
+				{
+					const size_t ki = (row_at + k0 + lane) * p.k_stride + col;
+					s = 0.0f;
+					for (int d = 0; d < hd; ++d) s = fmaf(el(p.q, qi + d), el(p.k, ki + d), s);
+					s *= p.scale * kLog2e;
+				}
+				float now = s;
+				for (int x = 1; x < 64; x *= 2) now = fmaxf(now, __shfl_xor(now, x));
+				now = fmaxf(now, m);
+				const float f = now == m ? 1.0f : fast_exp2(m - now), at = now == -INFINITY ? 0.0f : now;
+				m = now;
+				const float w = k0 + lane <= last ? fast_exp2(s - at) : 0.0f;
+				l = l * f + w;
+				for (int c = 0; c < kFlashMaxDim / 64; ++c) o[c] *= f;
+				for (int j = 0; j < 64 && k0 + j <= last; ++j)
+				{
+					const float wj = __shfl(w, j);
+					const size_t vi = (row_at + k0 + j) * p.v_stride + col;
+					for (int c = 0; c < kFlashMaxDim / 64; ++c)
+						if (64 * c + lane < hd) o[c] = fmaf(wj, el(p.v, vi + 64 * c + lane), o[c]);
+				}
+			}
+			for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
+			const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+			const size_t oi = (row_at + tok) * p.out_stride + static_cast<size_t>(head) * hd;
+			for (int c = 0; c < kFlashMaxDim / 64; ++c)
+			{
+				const int d = 64 * c + lane;
+				if (d >= hd) continue;
+				if constexpr (MODE == kBf16) static_cast<uint16_t*>(p.out)[oi + d] = static_cast<uint16_t>(cvt_pk_bf16(o[c] * inv, 0.0f));
+				else static_cast<float*>(p.out)[oi + d] = o[c] * inv;
+			}
+		}
+
+		template <int MODE, int HD, int NSEQ>
+		__global__ __launch_bounds__(64 * kWaves, (shape<MODE, HD>::PER_SIMD)) void flash_kernel(const flash_params p,
+		                                                                                      const flash_seqs<NSEQ> seqs)
+		{
+			using G = shape<MODE, HD>;
+			constexpr int KS = G::KS, KT = G::KT;
+			constexpr bool SPLIT = MODE != kBf16; // Q and P as hi + lo
+			typedef std::conditional_t<MODE == kBf16, bf16x8, f16x8> op8;
+			__shared__ __align__(16) unsigned char smem[G::BYTES];
+			__shared__ uint32_t s_max[2][kWaves];
+			uint16_t* const sk = reinterpret_cast<uint16_t*>(smem);
+			uint16_t* const sv = sk + G::PARTS * G::K_HALVES;
+
+			const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
+			const int hd = p.head_dim, group = p.n_head / p.n_kv;
+			const int kvh = static_cast<int>(blockIdx.x % p.n_kv), tile = static_cast<int>(blockIdx.x / p.n_kv);
+
+			// The sequence the tile belongs to: the last one whose tiles begin at or
+			// before it (every listed sequence has tiles).
+			int s_idx = 0;
+#pragma unroll
+			for (int c = 0; c < (NSEQ + 63) / 64; ++c)
+			{
+				const int i = 64 * c + lane;
+				s_idx += __popcll(__ballot(i < seqs.n && seqs.tile[i < NSEQ ? i : 0] <= tile));
+			}
+			s_idx = __builtin_amdgcn_readfirstlane(s_idx - 1);
+			const int len = seqs.len[s_idx];
+			const size_t row_at = static_cast<size_t>(seqs.start[s_idx]); // of the sequence's first token
+			const long long n_rows = static_cast<long long>(len) * group;
+			// (the last rows of a causal sequence have the most keys: they go first)
+			const int n_blk = static_cast<int>((n_rows + kRows - 1) / kRows);
+			const long long r0 = static_cast<long long>(n_blk - 1 - (tile - seqs.tile[s_idx])) * kRows;
+			const int pos0 = MODE == kQ4 ? p.pos0 : 0, n_keys = MODE == kQ4 ? p.n_seq : len;
+
+			auto token_of = [&](long long r) { return static_cast<int>((r < n_rows ? r : n_rows - 1) / group); };
+			auto span_of = [&](long long r, int& a, int& b) { attn_span(p.causal, p.window, pos0 + token_of(r), n_keys, a, b); };
+
+			// The lane's row, and the keys of the work-group's and the wavefront's rows.
+			const long long row = r0 + 32 * wave + r32;
+			const bool real = row < n_rows;
+			const int tok = token_of(row), head = kvh * group + (real ? static_cast<int>(row % group) : 0);
+			int first, last;
+			attn_span(p.causal, p.window, pos0 + tok, n_keys, first, last);
+			int kmin, kmax, wmin, wmax, full_from, full_to, unused;
+			span_of(r0, kmin, unused);
+			span_of(r0 + kRows - 1, unused, kmax);
+			span_of(r0 + 32 * wave, wmin, full_to); // every row of the wavefront sees full_from .. full_to
+			span_of(r0 + 32 * wave + 31, full_from, wmax);
+			const bool wave_real = r0 + 32 * wave < n_rows;
+
+			// ---- Q ----
+			constexpr int NQ = HD / 16;
+			op8 qh[NQ];
+			f16x8 ql[SPLIT ? NQ : 1];
+			// (S * sc in log2 units; the scale's sign goes into Q, so that a masked
+			// score stays the least whatever the scale)
+			float sc = fmaxf(fabsf(p.scale) * kLog2e, 1.17549435e-38f);
+			if constexpr (!SPLIT)
+			{
+				const uint16_t* q = static_cast<const uint16_t*>(p.q) + (row_at + tok) * p.q_stride + static_cast<size_t>(head) * hd;
+				const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+				for (int ks = 0; ks < NQ; ++ks)
+				{
+					const int d = 16 * ks + 8 * half;
+					u32x4 w = {0, 0, 0, 0};
+					if (d < hd) w = *reinterpret_cast<const u32x4*>(q + d) ^ u32x4{flip, flip, flip, flip};
+					qh[ks] = as_bf16x8(w);
+				}
+			}
+			else
+			{
+				const float* q = static_cast<const float*>(p.q) + (row_at + tok) * p.q_stride + static_cast<size_t>(head) * hd;
+				float x[NQ][8];
+				float m = 0.0f;
+#pragma unroll
+				for (int ks = 0; ks < NQ; ++ks)
+				{
+					const int d = 16 * ks + 8 * half;
+					float4 u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+					if (d < hd) u = *reinterpret_cast<const float4*>(q + d), v = *reinterpret_cast<const float4*>(q + d + 4);
+					if constexpr (MODE == kQ4) // (the k slot order of the 4-bit values)
+						x[ks][0] = u.x, x[ks][1] = v.x, x[ks][2] = u.y, x[ks][3] = v.y, x[ks][4] = u.z, x[ks][5] = v.z, x[ks][6] = u.w,
+						x[ks][7] = v.w;
+					else
+						x[ks][0] = u.x, x[ks][1] = u.y, x[ks][2] = u.z, x[ks][3] = u.w, x[ks][4] = v.x, x[ks][5] = v.y, x[ks][6] = v.z,
+						x[ks][7] = v.w;
+#pragma unroll
+					for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[ks][j]));
+				}
+				m = max_with_other_half(m);
+				// (0, infinity and NaN: as they are)
+				const int e = m > 0.0f && m < INFINITY ? up_to_2_15(__float_as_uint(m)) : 0;
+				const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+				sc = fmaxf(ldexpf(sc, -e), 1.17549435e-38f);
+#pragma unroll
+				for (int ks = 0; ks < NQ; ++ks)
+				{
+					u32x4 h, l;
+#pragma unroll
+					for (int j = 0; j < 4; ++j)
+					{
+						uint32_t a, b;
+						split_f16x2(sign * ldexpf(x[ks][2 * j], e), sign * ldexpf(x[ks][2 * j + 1], e), a, b);
+						h[j] = a;
+						l[j] = b;
+					}
+					qh[ks] = as_f16x8(h);
+					ql[ks] = as_f16x8(l);
+				}
+			}
+
+			// ---- the loads of a step ----
+			// Through buffer descriptors that end with the sequence's last row: keys
+			// past it read as zeros, and a thread's offsets are the same in every
+			// step (columns past head_dim: an offset past any descriptor).
+			constexpr int ESIZE = MODE == kBf16 ? 2 : 4;
+			const int blocks = hd / kQ4Block; // 4-bit: records of a KV head and group
+			// Key u of a V piece: set (tile, s, h), k slot order (keys 8 s + 4 h + j and
+			// 16 + 8 s + 4 h + j alternate).
+			constexpr uint32_t kNowhere = 0x80000000u;
+			uint32_t k_off[G::NK], v_off[G::NV];
+			if constexpr (MODE != kQ4)
+			{
+#pragma unroll
+				for (int n = 0; n < G::NK; ++n)
+				{
+					const int c = threadIdx.x + 256 * n, d = 8 * (c % (HD / 8));
+					k_off[n] = d < hd ? static_cast<uint32_t>((c / (HD / 8)) * p.k_stride + d) * ESIZE : kNowhere;
+				}
+#pragma unroll
+				for (int n = 0; n < G::NV; ++n)
+				{
+					const int c = threadIdx.x + 256 * n, set = c / (HD / 2), d = 2 * (c % (HD / 2));
+					const int key = 32 * (set >> 2) + 8 * ((set >> 1) & 1) + 4 * (set & 1);
+					v_off[n] = set < KS / 8 && d < hd ? static_cast<uint32_t>(key * p.v_stride + d) * ESIZE : kNowhere;
+				}
+			}
+			// Rows k0 .. of a tensor (at most KS of them, as far as the sequence goes).
+			auto rows_from = [&](const void* base, size_t stride, int k0)
+			{
+				const int n = n_keys - k0 < KS ? n_keys - k0 : KS;
+				const char* at = static_cast<const char*>(base) + ((row_at + k0) * stride + static_cast<size_t>(kvh) * hd) * ESIZE;
+				return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, static_cast<int>(((n - 1) * stride + hd) * ESIZE), kBufferFlags);
+			};
+			auto load_step = [&](int k0, step_regs<MODE, HD>& g)
+			{
+				if constexpr (MODE == kQ4)
+				{
+					const int groups = p.rows / kQ4Rows;
+#pragma unroll
+					for (int n = 0; n < G::NR; ++n)
+					{
+						const int rec = wave * G::NR + n, b = rec % (HD / 32), gi = rec / (HD / 32);
+						g.code[n] = u32x4{0, 0, 0, 0};
+						g.ksz[n] = u32x2{0, 0};
+						g.vs[n] = g.vz[n] = u32x4{0, 0, 0, 0};
+						if (gi >= KT || b >= blocks || k0 + 32 * gi > kmax) continue;
+						const unsigned char* at = static_cast<const unsigned char*>(p.k) +
+						                          (static_cast<size_t>((k0 / kQ4Rows + gi) % groups) * (p.n_kv * blocks) + kvh * blocks + b) * kQ4Record;
+						g.code[n] = *reinterpret_cast<const u32x4*>(at + 16 * lane);
+						g.ksz[n] = *reinterpret_cast<const u32x2*>(at + kQ4KScales + 8 * (lane & 15));
+						g.vs[n] = *reinterpret_cast<const u32x4*>(at + kQ4VScales + 32 * (lane >> 4));
+						g.vz[n] = *reinterpret_cast<const u32x4*>(at + kQ4VScales + 32 * (lane >> 4) + 16);
+					}
+				}
+				else
+				{
+					const auto rk = rows_from(p.k, p.k_stride, k0), rv = rows_from(p.v, p.v_stride, k0);
+#pragma unroll
+					for (int n = 0; n < G::NK; ++n)
+#pragma unroll
+						for (int x = 0; x < G::PARTS; ++x)
+							g.k[G::PARTS * n + x] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off[n] + 16 * x, 0, 0));
+					const uint32_t row_bytes = static_cast<uint32_t>(p.v_stride * ESIZE);
+#pragma unroll
+					for (int n = 0; n < G::NV; ++n)
+#pragma unroll
+						for (int u = 0; u < 8; ++u)
+						{
+							// (in the checked offset: a scalar one would be taken off the bound)
+							const uint32_t at = v_off[n] + ((u >> 1) + 16 * (u & 1)) * row_bytes;
+							if constexpr (MODE == kBf16)
+								g.v[n][u] = __builtin_amdgcn_raw_buffer_load_b32(rv, at, 0, 0);
+							else
+							{
+								const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, at, 0, 0));
+								g.v[n][2 * u] = w.x;
+								g.v[n][2 * u + 1] = w.y;
+							}
+						}
+				}
+			};
+
+			// The registers' K rows and V^T rows into LDS (F32: times 2^ek, 2^ev).
+			auto store_step = [&](const step_regs<MODE, HD>& g, int ek, int ev)
+			{
+				if constexpr (MODE == kQ4)
+				{
+#pragma unroll
+					for (int n = 0; n < G::NR; ++n)
+					{
+						const int rec = wave * G::NR + n, b = rec % (HD / 32), gi = rec / (HD / 32);
+						if (gi >= KT) continue;
+						const int i = lane & 15, q = lane >> 4;
+#pragma unroll
+						for (int t = 0; t < 2; ++t)
+						{
+							const f16x8 x = q4_k(t ? g.code[n].y : g.code[n].x, t ? g.ksz[n].y : g.ksz[n].x);
+							*reinterpret_cast<f16x8*>(sk + (32 * gi + 16 * t + i) * G::KP + 32 * b + 8 * q) = x;
+							// (quarter q of the rows: rows 4 q + j and 16 + 4 q + j, i.e. s = q / 2, h = q % 2)
+							const f16x8 y = q4_v(t ? g.code[n].w : g.code[n].z, g.vs[n], g.vz[n]);
+							*reinterpret_cast<f16x8*>(sv + (32 * b + 16 * t + i) * G::VP + 32 * gi + 8 * q) = y;
+						}
+					}
+				}
+				else if constexpr (MODE == kBf16)
+				{
+#pragma unroll
+					for (int n = 0; n < G::NK; ++n)
+					{
+						const int c = threadIdx.x + 256 * n;
+						*reinterpret_cast<u32x4*>(sk + c / (HD / 8) * G::KP + 8 * (c % (HD / 8))) = g.k[n];
+					}
+#pragma unroll
+					for (int n = 0; n < G::NV; ++n)
+					{
+						const int c = threadIdx.x + 256 * n, set = c / (HD / 2), d = 2 * (c % (HD / 2));
+						if (set >= KS / 8) continue;
+						u32x4 a, b; // columns d and d + 1
+#pragma unroll
+						for (int j = 0; j < 4; ++j)
+						{
+							a[j] = __builtin_amdgcn_perm(g.v[n][2 * j + 1], g.v[n][2 * j], 0x05040100u);
+							b[j] = __builtin_amdgcn_perm(g.v[n][2 * j + 1], g.v[n][2 * j], 0x07060302u);
+						}
+						*reinterpret_cast<u32x4*>(sv + d * G::VP + 8 * set) = a;
+						*reinterpret_cast<u32x4*>(sv + (d + 1) * G::VP + 8 * set) = b;
+					}
+				}
+				else
+				{
+#pragma unroll
+					for (int n = 0; n < G::NK; ++n)
+					{
+						const int c = threadIdx.x + 256 * n;
+						u32x4 h, l;
+#pragma unroll
+						for (int j = 0; j < 4; ++j)
+						{
+							const u32x4 w = g.k[2 * n + (j >> 1)];
+							uint32_t a, b;
+							split_f16x2(ldexpf(__uint_as_float(w[2 * (j & 1)]), ek), ldexpf(__uint_as_float(w[2 * (j & 1) + 1]), ek), a, b);
+							h[j] = a;
+							l[j] = b;
+						}
+						uint16_t* at = sk + c / (HD / 8) * G::KP + 8 * (c % (HD / 8));
+						*reinterpret_cast<u32x4*>(at) = h;
+						*reinterpret_cast<u32x4*>(at + G::K_HALVES) = l;
+					}
+#pragma unroll
+					for (int n = 0; n < G::NV; ++n)
+					{
+						const int c = threadIdx.x + 256 * n, set = c / (HD / 2), d = 2 * (c % (HD / 2));
+						if (set >= KS / 8) continue;
+#pragma unroll
+						for (int col = 0; col < 2; ++col)
+						{
+							u32x4 h, l;
+#pragma unroll
+							for (int j = 0; j < 4; ++j)
+							{
+								uint32_t a, b;
+								split_f16x2(ldexpf(__uint_as_float(g.v[n][4 * j + col]), ev), ldexpf(__uint_as_float(g.v[n][4 * j + 2 + col]), ev), a, b);
+								h[j] = a;
+								l[j] = b;
+							}
+							uint16_t* at = sv + (d + col) * G::VP + 8 * set;
+							*reinterpret_cast<u32x4*>(at) = h;
+							*reinterpret_cast<u32x4*>(at + G::V_HALVES) = l;
+						}
+					}
+				}
+			};
+
+			// ---- the walk ----
+			f32x16 o[HD / 32] = {};
+			float off = -INFINITY, l = 0.0f;
+			int ev = 1000; // F32: O is in units of 2^-ev (1000: nothing added yet)
+			// (raises the offset for a largest score m, in log2 units)
+			auto raise = [&](float m)
+			{
+				const bool up = m > off + kRaise;
+				if (__any(up))
+				{
+					const float now = up ? m - kBelow : off;
+					// (equal ones first: -inf - -inf is NaN)
+					const float f = now == off ? 1.0f : fast_exp2(off - now);
+					off = now;
+					l *= f;
+#pragma unroll
+					for (int dt = 0; dt < HD / 32; ++dt) o[dt] *= f;
+				}
+			};
+
+			bool by_vector = false;
+			step_regs<MODE, HD> regs;
+			const int k_first = kmin / KS * KS;
+			if (k_first <= kmax) load_step(k_first, regs);
+			for (int k0 = k_first; k0 <= kmax; k0 += KS)
+			{
+				// Largest magnitudes (F32), or whether V holds an infinite or NaN element
+				// (BF16, masked steps).
+				bool slow = false;
+				int ek = 0;
+				if constexpr (MODE == kF32)
+				{
+					uint32_t mk = 0, mv = 0;
+#pragma unroll
+					for (int n = 0; n < 2 * G::NK; ++n)
+#pragma unroll
+						for (int j = 0; j < 4; ++j) mk = umax(mk, regs.k[n][j] & 0x7fffffffu);
+#pragma unroll
+					for (int n = 0; n < G::NV; ++n)
+#pragma unroll
+						for (int j = 0; j < 16; ++j) mv = umax(mv, regs.v[n][j] & 0x7fffffffu);
+					mk = wave_umax(mk);
+					mv = wave_umax(mv);
+					if (lane == 0) s_max[0][wave] = mk, s_max[1][wave] = mv;
+				}
+				else if constexpr (MODE == kBf16)
+				{
+					int a, b;
+					span_of(r0, unused, b);
+					span_of(r0 + kRows - 1, a, unused);
+					if (k0 < a || k0 + KS - 1 > b) // some row of the work-group does not see them all
+					{
+						bool bad = false;
+#pragma unroll
+						for (int n = 0; n < G::NV; ++n)
+#pragma unroll
+							for (int u = 0; u < 8; ++u)
+								bad |= (regs.v[n][u] & 0x7f80u) == 0x7f80u || (regs.v[n][u] & 0x7f800000u) == 0x7f800000u;
+						if (lane == 0) s_max[0][wave] = 0;
+						if (__any(bad) && lane == 0) s_max[0][wave] = 1;
+						slow = true; // (to be looked at)
+					}
+				}
+				__syncthreads(); // every wavefront is done with the step before
+				if constexpr (MODE == kF32)
+				{
+					uint32_t mk = 0, mv = 0;
+#pragma unroll
+					for (int w = 0; w < kWaves; ++w) mk = umax(mk, s_max[0][w]), mv = umax(mv, s_max[1][w]);
+					slow = mk >= 0x7f800000u || mv >= 0x7f800000u;
+					if (!slow)
+					{
+						ek = up_to_2_15(mk);
+						const int want = mv == 0 ? ev : up_to_2_15(mv);
+						if (want < ev) // (V grows: O follows)
+						{
+							if (ev != 1000)
+#pragma unroll
+								for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+									for (int i = 0; i < 16; ++i) o[dt][i] = ldexpf(o[dt][i], want - ev);
+							ev = want;
+						}
+					}
+				}
+				else if constexpr (MODE == kBf16)
+				{
+					if (slow) slow = (s_max[0][0] | s_max[0][1] | s_max[0][2] | s_max[0][3]) != 0;
+				}
+				if (MODE != kQ4 && __builtin_amdgcn_readfirstlane(slow))
+				{
+					by_vector = true; // (the whole work-group)
+					break;
+				}
+
+				store_step(regs, ek, ev);
+				if (k0 + KS <= kmax) load_step(k0 + KS, regs);
+				__syncthreads();
+				if (!wave_real || k0 > wmax || k0 + KS - 1 < wmin) continue;
+
+				f32x16 s[KT] = {};
+#pragma unroll
+				for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+					for (int ks = 0; ks < NQ; ++ks)
+					{
+						const uint16_t* at = sk + (32 * kt + r32) * G::KP + 16 * ks + 8 * half;
+						const op8 a = *reinterpret_cast<const op8*>(at);
+						s[kt] = mfma32x32x16(a, qh[ks], s[kt]);
+						if constexpr (SPLIT) s[kt] = mfma32x32x16(a, ql[ks], s[kt]);
+						if constexpr (MODE == kF32) s[kt] = mfma32x32x16(*reinterpret_cast<const op8*>(at + G::K_HALVES), qh[ks], s[kt]);
+					}
+				float f = sc;
+				if constexpr (MODE == kF32) f = fminf(fmaxf(ldexpf(sc, -ek), 1.17549435e-38f), 1e36f);
+				if (k0 < full_from || k0 + KS - 1 > full_to)
+#pragma unroll
+					for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+						for (int i = 0; i < 16; ++i)
+						{
+							const int key = k0 + 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3);
+							if (key < first || key > last) s[kt][i] = -INFINITY;
+						}
+				float m = s[0][0];
+#pragma unroll
+				for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+					for (int i = 0; i < 16; ++i) m = fmaxf(m, s[kt][i]);
+				raise(max_with_other_half(m) * f);
+				const float at = off == -INFINITY ? 0.0f : off;
+#pragma unroll
+				for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+					for (int i = 0; i < 16; ++i)
+					{
+						s[kt][i] = fast_exp2(fmaf(s[kt][i], f, -at));
+						l += s[kt][i];
+					}
+#pragma unroll
+				for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+					for (int h = 0; h < 2; ++h)
+					{
+						u32x4 wh, wl;
+#pragma unroll
+						for (int j = 0; j < 4; ++j)
+						{
+							const float a = s[kt][4 * h + j], b = s[kt][8 + 4 * h + j];
+							if constexpr (SPLIT)
+							{
+								uint32_t x, y;
+								split_weights(a, b, x, y);
+								wh[j] = x;
+								wl[j] = y;
+							}
+							else
+								wh[j] = cvt_pk_bf16(a, b);
+						}
+						const op8 ph = __builtin_bit_cast(op8, wh);
+#pragma unroll
+						for (int dt = 0; dt < HD / 32; ++dt)
+						{
+							const uint16_t* v = sv + (32 * dt + r32) * G::VP + 32 * kt + 16 * h + 8 * half;
+							const op8 a = *reinterpret_cast<const op8*>(v);
+							o[dt] = mfma32x32x16(a, ph, o[dt]);
+							if constexpr (SPLIT) o[dt] = mfma32x32x16(a, __builtin_bit_cast(op8, wl), o[dt]);
+							if constexpr (MODE == kF32) o[dt] = mfma32x32x16(*reinterpret_cast<const op8*>(v + G::V_HALVES), ph, o[dt]);
+						}
+					}
+			}
+
+			if constexpr (MODE != kQ4)
+				if (by_vector)
+				{
+					for (int r = 0; r < 32 && r0 + 32 * wave + r < n_rows; ++r)
+					{
+						const long long x = r0 + 32 * wave + r;
+						int a, b;
+						span_of(x, a, b);
+						vector_row<MODE>(p, row_at, token_of(x), kvh * group + static_cast<int>(x % group), kvh, a, b, lane);
+					}
+					return;
+				}
+
+			// ---- out ----
+			l = add_with_other_half(l);
+			if (!real) return;
+			const float inv = l == 0.0f ? 0.0f : 1.0f / l; // (a row that sees nothing: zeros)
+			const size_t oi = (row_at + tok) * p.out_stride + static_cast<size_t>(head) * hd;
+#pragma unroll
+			for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+				for (int c = 0; c < 4; ++c)
+				{
+					const int d = 32 * dt + 8 * c + 4 * half;
+					if (d >= hd) continue;
+					float y[4];
+#pragma unroll
+					for (int j = 0; j < 4; ++j)
+					{
+						y[j] = o[dt][4 * c + j] * inv;
+						if constexpr (MODE == kF32) y[j] = ldexpf(y[j], ev == 1000 ? 0 : -ev);
+						if constexpr (MODE == kQ4) y[j] = gated(y[j], p.gate, oi + d + j);
+					}
+					if constexpr (MODE == kBf16)
+						*reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + oi + d) = u32x2{cvt_pk_bf16(y[0], y[1]), cvt_pk_bf16(y[2], y[3])};
+					else
+						*reinterpret_cast<float4*>(static_cast<float*>(p.out) + oi + d) = float4{y[0], y[1], y[2], y[3]};
+				}
+		}
+
+		template <int MODE, int NSEQ>
+		bool launch_mode(const flash_params& p, const flash_seqs<NSEQ>& s, hipStream_t stream)
+		{
+			const unsigned long long wg = static_cast<unsigned long long>(s.tiles) * p.n_kv;
+			if (wg > 0x7fffffffull) return false;
+			const dim3 grid(static_cast<unsigned>(wg));
+			if (p.head_dim <= 64)
+				flash_kernel<MODE, 64, NSEQ><<<grid, 64 * kWaves, 0, stream>>>(p, s);
+			else if (p.head_dim <= 96)
+				flash_kernel<MODE, 96, NSEQ><<<grid, 64 * kWaves, 0, stream>>>(p, s);
+			else if (p.head_dim <= 128)
+				flash_kernel<MODE, 128, NSEQ><<<grid, 64 * kWaves, 0, stream>>>(p, s);
+			else
+				flash_kernel<MODE, 256, NSEQ><<<grid, 64 * kWaves, 0, stream>>>(p, s);
+			return true;
+		}
+	}
+
+	int flash_tiles(int len, int group) { return static_cast<int>((static_cast<long long>(len) * group + kRows - 1) / kRows); }
+
+	bool launch_packed(const flash_params& p, const flash_seqs<kFlashSeqs>& s, bool bf16, hipStream_t stream)
+	{
+		return bf16 ? launch_mode<kBf16>(p, s, stream) : launch_mode<kF32>(p, s, stream);
+	}
+
+	bool launch_flash_q4(const flash_params& p, int n_tok, hipStream_t stream)
+	{
+		flash_seqs<1> s{};
+		s.n = 1;
+		s.len[0] = n_tok;
+		s.tiles = flash_tiles(n_tok, p.n_head / p.n_kv);
+		return launch_mode<kQ4>(p, s, stream);
+	}
+}

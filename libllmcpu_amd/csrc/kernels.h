@@ -149,6 +149,36 @@ namespace nnchip
 	void launch_read_rows(const void* K, const void* V, float* k_out, float* v_out, size_t first, size_t n, bool bf16,
 	                      hipStream_t stream);
 
+	// Attention of many rows over whole sequences (attn_flash.hip): packed
+	// prompts, and batches over the 4-bit cache.
+	struct flash_params
+	{
+		// packed: rows of the element type, *_stride elements apart, head h at
+		// column h * head_dim; 4-bit: F32 q and out, k the records
+		const void* q;
+		const void* k;
+		const void* v;
+		void* out;
+		const float* gate; // 4-bit: [n_tok][n_head * head_dim], or null
+		size_t q_stride, k_stride, v_stride, out_stride;
+		int n_head, n_kv, head_dim; // packed: head_dim a multiple of 8, at most kFlashMaxDim
+		int causal, window;
+		float scale;
+		int pos0, n_seq, rows; // 4-bit: position of the first row, keys, rows of the buffer
+	};
+	constexpr int kFlashMaxDim = 256;
+	// Sequences of one launch, none of them empty: first row, length, first tile.
+	constexpr int kFlashSeqs = 64;
+	template <int N>
+	struct flash_seqs
+	{
+		int n, tiles;
+		int start[N], len[N], tile[N];
+	};
+	int flash_tiles(int len, int group); // row blocks of a sequence
+	bool launch_packed(const flash_params& p, const flash_seqs<kFlashSeqs>& s, bool bf16, hipStream_t stream);
+	bool launch_flash_q4(const flash_params& p, int n_tok, hipStream_t stream);
+
 	// Tiled MFMA attention for a batch of query tokens.
 	struct prefill_params
 	{

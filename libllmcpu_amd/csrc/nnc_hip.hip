@@ -804,6 +804,31 @@ namespace
 		const int kmin = first0, kmax = last1;
 		if (kmax < kmin) return nnchip::launch_zero(out, q_floats, kv->stream) ? NNC_OK : NNC_ERR_IO;
 
+		// A batch over a 4-bit cache: the tiled MFMA kernel, out of exact mode (at
+		// head_dim 512 the split-K kernels).
+		if (kv->q4 && n_tok > kSessionBatch && !kv->exact_batches && head_dim <= nnchip::kFlashMaxDim)
+		{
+			nnchip::flash_params p{};
+			p.q = q;
+			p.k = b.k;
+			p.out = out;
+			p.gate = gate;
+			p.q_stride = p.out_stride = static_cast<size_t>(n_head) * head_dim;
+			p.n_head = n_head;
+			p.n_kv = n_kv;
+			p.head_dim = head_dim;
+			p.causal = causal ? 1 : 0;
+			p.window = window;
+			p.scale = scale;
+			p.pos0 = pos0;
+			p.n_seq = n_seq;
+			p.rows = b.rows;
+			if (!nnchip::launch_flash_q4(p, n_tok, kv->stream))
+				return fail(NNC_ERR_UNSUPPORTED_MODEL, "%d tokens of %d heads are too many for one call", n_tok, n_head);
+			NNC_HIP_TRY(hipGetLastError(), "attention over a 4-bit cache");
+			return NNC_OK;
+		}
+
 		// Decode and session-sized batches (and every batch in exact mode):
 		// the split-K kernels, each token on its own split grid. Larger
 		// batches: the MFMA prefill kernel for BF16 K/V of its head shapes;
@@ -1327,6 +1352,96 @@ nnc_status nnc_hip_attend_gated_device(nnc_hip_kv* kv, int32_t buf, const float*
 	if (nnc_status s = check_attend(kv, buf, q, out, n_tok, pos0, n_seq, window, causal, n_head, n_kv, head_dim))
 		return s;
 	return attend_impl(kv, buf, q, out, gate, n_tok, pos0, n_seq, window, causal, n_head, n_kv, head_dim, scale);
+}
+
+nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void* q, size_t q_stride, const void* k,
+                                        size_t k_stride, const void* v, size_t v_stride, void* out, size_t out_stride,
+                                        const int32_t* starts, int32_t n_seqs, int32_t window, bool causal, int32_t n_head,
+                                        int32_t n_kv, int32_t head_dim, float scale)
+{
+	if (!kv) return fail(NNC_ERR_INVALID_ARGUMENT, "the cache is NULL");
+	if (type != NNC_HIP_F32 && type != NNC_HIP_BF16) return fail(NNC_ERR_INVALID_ARGUMENT, "element type %d", type);
+	if (!q || !k || !v || !out) return fail(NNC_ERR_INVALID_ARGUMENT, "NULL q, k, v or out");
+	if (n_seqs < 0 || (n_seqs > 0 && !starts) || window < 0)
+		return fail(NNC_ERR_INVALID_ARGUMENT, "%d sequences, starts %s, window %d", n_seqs, starts ? "given" : "NULL", window);
+	if (n_kv <= 0 || n_head <= 0 || n_head % n_kv != 0 || head_dim <= 0)
+		return fail(NNC_ERR_INVALID_ARGUMENT, "bad heads: %d query heads over %d KV heads, head_dim %d", n_head, n_kv, head_dim);
+	if (head_dim % 8 != 0 || head_dim > nnchip::kFlashMaxDim)
+		return fail(NNC_ERR_UNSUPPORTED_MODEL, "head_dim %d is not supported for packed sequences (a multiple of 8 up to %d)",
+		            head_dim, nnchip::kFlashMaxDim);
+	if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+	     reinterpret_cast<uintptr_t>(out)) & 15)
+		return fail(NNC_ERR_INVALID_ARGUMENT, "q, k, v and out must be 16-byte aligned");
+	const size_t q_dim = static_cast<size_t>(n_head) * head_dim, kv_dim = static_cast<size_t>(n_kv) * head_dim;
+	const size_t step = type == NNC_HIP_BF16 ? 8 : 4, most = size_t{1} << 23; // (a step's rows: 32-bit byte offsets)
+	if (q_stride < q_dim || out_stride < q_dim || k_stride < kv_dim || v_stride < kv_dim ||
+	    (q_stride | out_stride | k_stride | v_stride) % step != 0 || (q_stride | out_stride | k_stride | v_stride) >= most)
+		return fail(NNC_ERR_INVALID_ARGUMENT,
+		            "row strides %zu, %zu, %zu, %zu: at least the row's %zu or %zu elements, multiples of %zu, under %zu", q_stride,
+		            k_stride, v_stride, out_stride, q_dim, kv_dim, step, most);
+	for (int32_t i = 0; i < n_seqs; ++i)
+		if (starts[0] < 0 || starts[i + 1] < starts[i])
+			return fail(NNC_ERR_INVALID_ARGUMENT, "sequence %d: rows %d up to %d", i, starts[i], starts[i + 1]);
+
+	// The longest first, kFlashSeqs to a launch, so that no long tile is begun
+	// last.
+	const int group = n_head / n_kv;
+	std::vector<int32_t> order;
+	try
+	{
+		order.reserve(static_cast<size_t>(n_seqs));
+	}
+	catch (const std::bad_alloc&)
+	{
+		return fail(NNC_ERR_OUT_OF_MEMORY, "out of host memory");
+	}
+	for (int32_t i = 0; i < n_seqs; ++i)
+		if (starts[i + 1] > starts[i]) order.push_back(i);
+	std::sort(order.begin(), order.end(), [&](int32_t a, int32_t b)
+	{
+		const int32_t la = starts[a + 1] - starts[a], lb = starts[b + 1] - starts[b];
+		return la != lb ? la > lb : a < b;
+	});
+	nnchip::flash_params p{};
+	p.q = q;
+	p.k = k;
+	p.v = v;
+	p.out = out;
+	p.q_stride = q_stride;
+	p.k_stride = k_stride;
+	p.v_stride = v_stride;
+	p.out_stride = out_stride;
+	p.n_head = n_head;
+	p.n_kv = n_kv;
+	p.head_dim = head_dim;
+	p.causal = causal ? 1 : 0;
+	p.window = window;
+	p.scale = scale;
+	// Counted before the first launch, so that a refused call changes nothing.
+	for (size_t at = 0; at < order.size(); at += nnchip::kFlashSeqs)
+	{
+		unsigned long long tiles = 0;
+		for (size_t i = at; i < std::min(at + nnchip::kFlashSeqs, order.size()); ++i)
+			tiles += nnchip::flash_tiles(starts[order[i] + 1] - starts[order[i]], group);
+		if (tiles * n_kv > INT_MAX)
+			return fail(NNC_ERR_UNSUPPORTED_MODEL, "%llu row blocks of %d KV heads are too many for one launch", tiles, n_kv);
+	}
+	const device_scope on(kv->device);
+	for (size_t at = 0; at < order.size(); at += nnchip::kFlashSeqs)
+	{
+		nnchip::flash_seqs<nnchip::kFlashSeqs> s{};
+		for (size_t i = at; i < std::min(at + nnchip::kFlashSeqs, order.size()); ++i, ++s.n)
+		{
+			s.start[s.n] = starts[order[i]];
+			s.len[s.n] = starts[order[i] + 1] - starts[order[i]];
+			s.tile[s.n] = s.tiles;
+			s.tiles += nnchip::flash_tiles(s.len[s.n], group);
+		}
+		if (!nnchip::launch_packed(p, s, type == NNC_HIP_BF16, kv->stream))
+			return fail(NNC_ERR_UNSUPPORTED_MODEL, "too many row blocks for one launch");
+		NNC_HIP_TRY(hipGetLastError(), "packed attention");
+	}
+	return NNC_OK;
 }
 
 namespace

@@ -137,6 +137,8 @@ SIGNATURES = {
     "nnc_hip_attend_device_noalloc": (C.c_int, [_P, _I, _P, _P, _I, _I, _I, _I, _B, _I, _I, _I, _F]),
     "nnc_hip_attend_gated": (C.c_int, [_P, _I, _P, _P, _P, _I, _I, _I, _I, _B, _I, _I, _I, _F]),
     "nnc_hip_attend_gated_device": (C.c_int, [_P, _I, _P, _P, _P, _I, _I, _I, _I, _B, _I, _I, _I, _F]),
+    "nnc_hip_attend_packed_device": (C.c_int, [_P, _I, _P, C.c_size_t, _P, C.c_size_t, _P, C.c_size_t, _P, C.c_size_t,
+                                               C.POINTER(_I), _I, _I, _B, _I, _I, _I, _F]),
     "nnc_hip_gemv_bf16": (C.c_int, [_P, _P, _P, C.c_size_t, _P, C.c_size_t, C.c_uint32, C.c_uint32, C.c_uint32]),
     "nnc_hip_gemv_bf16_argmax": (C.c_int, [_P, _P, _P, C.c_uint32, C.c_uint32, C.POINTER(C.c_int32)]),
     "nnc_hip_argmax_f32": (C.c_int, [_P, _P, C.c_uint32, C.POINTER(C.c_int32)]),
@@ -396,6 +398,44 @@ class KVCache:
             n_seq = pos0 + n_tok
         _check(self._lib.nnc_hip_attend_device_noalloc(self.handle, buf, q_dev, out_dev, n_tok, pos0, n_seq, window,
                                                        bool(causal), n_head, n_kv, head_dim, float(scale)))
+
+    def attend_packed_device(self, q_dev: int, k_dev: int, v_dev: int, out_dev: int, *, starts, bf16: bool, n_head: int,
+                             n_kv: int, head_dim: int, scale: float, window: int = 0, causal: bool = True,
+                             q_stride: int | None = None, k_stride: int | None = None, v_stride: int | None = None,
+                             out_stride: int | None = None) -> None:
+        """Attention over whole sequences laid end to end (rows starts[s] ..
+        starts[s + 1] - 1 each, device addresses, BF16 or float32; strides in
+        elements), this cache the execution context; queued on its stream."""
+        n = len(starts)
+        arr = starts if isinstance(starts, C.Array) else (_I * n)(*starts)
+        qd, kd = n_head * head_dim, n_kv * head_dim
+        _check(self._lib.nnc_hip_attend_packed_device(
+            self.handle, int(bool(bf16)), q_dev, qd if q_stride is None else q_stride, k_dev,
+            kd if k_stride is None else k_stride, v_dev, kd if v_stride is None else v_stride, out_dev,
+            qd if out_stride is None else out_stride, arr, n - 1, window, bool(causal), n_head, n_kv, head_dim,
+            float(scale)))
+
+    def attend_packed(self, q: np.ndarray, k: np.ndarray, v: np.ndarray, *, starts, n_head: int, n_kv: int, head_dim: int,
+                      scale: float, window: int = 0, causal: bool = True) -> np.ndarray:
+        """attend_packed_device of host arrays (float32, or uint16 BF16 bits; through
+        scratch device memory, freed afterwards); rows in no sequence are zeros."""
+        from . import hip_rt
+
+        q, k, v = (np.ascontiguousarray(x) for x in (q, k, v))
+        if q.dtype not in (np.float32, np.uint16) or k.dtype != q.dtype or v.dtype != q.dtype:
+            raise ValueError("q, k and v are float32, or uint16 BF16 bits")
+        out, dev = np.zeros_like(q), []
+        try:
+            for a in (q, k, v, out):
+                dev.append(hip_rt.malloc(max(a.nbytes, 16)))
+                hip_rt.to_device(dev[-1], a)
+            self.attend_packed_device(*dev, starts=starts, bf16=q.dtype == np.uint16, n_head=n_head, n_kv=n_kv,
+                                      head_dim=head_dim, scale=scale, window=window, causal=causal)
+            self.sync()
+            return hip_rt.to_host(out, dev[3])
+        finally:
+            for p in dev:
+                hip_rt.free(p)
 
     def prep_append_device(self, buf: int, q_dev: int, k_dev: int, v_dev: int, *, pos0: int, n_tok: int,
                            prep: NncHipPrep) -> None:

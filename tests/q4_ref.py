@@ -43,8 +43,8 @@ def span(causal: bool, window: int, pos: int, n_seq: int):
 
 
 def attend(q, k, v, *, pos0, n_seq, window, causal, n_head, n_kv, head_dim, scale):
-    """(out, bound) of q [n_tok, n_head * head_dim] over the keys of positions 0 ..
-    n_seq - 1, both float64. bound: how far an output computed with fp32 sums and
+    """(out, bound, mean |V|) of q [n_tok, n_head * head_dim] over the keys of positions 0 ..
+    n_seq - 1, float64. bound: how far an output computed with fp32 sums and
     operands of 22 significant bits may be off. A score's products sum to at most
     A = scale max_k sum |q k|; their sum has the operands' roundings (2^-23 each)
     and a rounding of 2^-24 per partial sum, of which the matrix cores make two
@@ -53,7 +53,7 @@ def attend(q, k, v, *, pos0, n_seq, window, causal, n_head, n_kv, head_dim, scal
     output by twice its weights' relative error times the largest |V|."""
     n_tok, g = q.shape[0], n_head // n_kv
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
-    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    out, bound, spread = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape)
     for t in range(n_tok):
         first, last = span(causal, window, pos0 + t, n_seq)
         if last < first:
@@ -65,6 +65,7 @@ def attend(q, k, v, *, pos0, n_seq, window, causal, n_head, n_kv, head_dim, scal
                 s = kk @ q[t, at] * scale
                 w = np.exp(s - s.max())
                 out[t, at] = w @ vv / w.sum()
-                a = (np.abs(kk) @ np.abs(q[t, at])).max() * scale
+                spread[t, at] = w @ np.abs(vv) / w.sum()
+                a = (np.abs(kk) @ np.abs(q[t, at])).max() * abs(scale)
                 bound[t, at] = 2 * np.abs(vv).max() * (a * (head_dim / 16 + 8) * 2.0**-24 + 2.0**-21)
-    return out, bound
+    return out, bound, spread

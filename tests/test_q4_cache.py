@@ -198,7 +198,7 @@ def test_attention(n_head, n_kv, hd, rows, n_seq, pos0, n_tok, window, causal):
         got = kv.attend(0, q, pos0=pos0, n_seq=n_seq, **shape)
         gate = rows_of(10, n_tok, n_head * hd)
         gated = kv.attend(0, q, pos0=pos0, n_seq=n_seq, gate=gate, **shape)
-    want, bound = ref.attend(q, k, v, pos0=pos0, n_seq=n_seq, **shape)
+    want, bound, _ = ref.attend(q, k, v, pos0=pos0, n_seq=n_seq, **shape)
     d = np.abs(got - want)
     assert (d <= bound).all(), f"{d.max():.3g}, {(d / bound).max():.3g} of the bound"
     sig = 1 / (1 + np.exp(-gate.astype(np.float64)))
@@ -243,14 +243,14 @@ def test_tokens_that_see_nothing_and_large_scores():
         shape = dict(window=2, causal=True, n_head=4, n_kv=2, head_dim=hd, scale=0.125)
         q = rows_of(4, 3, 4 * hd)
         got = kv.attend(0, q, pos0=3, n_seq=3, **shape)
-        want, bound = ref.attend(q, k, v, pos0=3, n_seq=3, **shape)
+        want, bound, _ = ref.attend(q, k, v, pos0=3, n_seq=3, **shape)
         assert not got[1:].any() and (np.abs(got - want) <= bound).all()
         # scores of thousands, of both signs, and none at all
         shape = dict(window=0, causal=True, n_head=4, n_kv=2, head_dim=hd, scale=0.125)
         for f in (3000.0, 1e-30, 0.0):
             q = rows_of(5, 2, 4 * hd) * np.float32(f)
             got = kv.attend(0, q, pos0=298, **shape)
-            want, bound = ref.attend(q, k, v, pos0=298, n_seq=300, **shape)
+            want, bound, _ = ref.attend(q, k, v, pos0=298, n_seq=300, **shape)
             assert (np.abs(got - want) <= bound).all(), f
         # one token's q is NaN, and one infinite: the others' rows are untouched
         q = rows_of(6, 4, 4 * hd)
@@ -278,7 +278,7 @@ def test_long_cache_past_32_bits():
         for m in (1, 20):
             q = rows_of(3, m, dim)
             out = kv.attend(0, q, pos0=rows - m, **shape)
-            want, bound = ref.attend(q, kq, vq, pos0=n - m, n_seq=n, **shape)
+            want, bound, _ = ref.attend(q, kq, vq, pos0=n - m, n_seq=n, **shape)
             assert (np.abs(out - want) <= bound).all()
 
 
