@@ -41,6 +41,13 @@ namespace nnchip
 			const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
 			return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 		}
+		__device__ __forceinline__ float row_max(float x) // over 16 lanes
+		{
+			x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xf, 0xf, false)));
+			x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xf, 0xf, false)));
+			x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xf, 0xf, false)));
+			return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xf, 0xf, false)));
+		}
 		// Over the four lanes of a column.
 		__device__ __forceinline__ float column_max(float x) { return max_with_other_half(max_other_row(x)); }
 		__device__ __forceinline__ float column_sum(float x) { return add_with_other_half(add_with_other_row(x)); }
@@ -84,6 +91,31 @@ namespace nnchip
 
 			__shared__ float s_o[kW][8][HD + 4]; // a tile's outputs (relative to its offset), offset, sum
 
+			// The keys any pair of the launch attends to, within the split.
+			int kmin, kmax, unused;
+			attn_span(p.causal, p.window, p.pos0, p.n_seq, kmin, unused);
+			attn_span(p.causal, p.window, p.pos0 + p.n_tok - 1, p.n_seq, unused, kmax);
+			const int k0 = p.split_base + split * p.split_keys;
+			const int g_first = (kmin > k0 ? kmin : k0) / kQ4Rows;
+			const int g_last = (kmax < k0 + p.split_keys - 1 ? kmax : k0 + p.split_keys - 1) / kQ4Rows;
+			const int row_groups = p.rows / kQ4Rows, blocks = p.kv_dim / kQ4Block;
+			const unsigned char* recs = static_cast<const unsigned char*>(p.K) + static_cast<size_t>(kvh) * NB * kQ4Record;
+			const size_t group_bytes = static_cast<size_t>(blocks) * kQ4Record;
+			// (wavefront w takes the groups whose number in the split is w modulo kW)
+			int kg = k0 / kQ4Rows + wave;
+			if (kg < g_first) kg += (g_first - kg + kW - 1) / kW * kW;
+
+			// Up to 8 blocks the next group's records are in flight during the work on
+			// this one; 16 blocks' registers do not fit twice, and they are loaded here.
+			constexpr bool kAhead = NB <= 8;
+			auto records_of = [&](int n, record* r)
+			{
+#pragma unroll
+				for (int b = 0; b < NB; ++b)
+					r[b] = load_record(recs + static_cast<size_t>(n % row_groups) * group_bytes + b * kQ4Record, lane);
+			};
+			record r[NB];
+			if (kAhead && kg <= g_last) records_of(kg, r);
 			// Q: per pair brought under 2^15 by a power of two, then fp16 hi or lo.
 			f16x8 q[T][NB];
 			float back[T]; // 2^-that power, and log2(e) * scale
@@ -128,31 +160,6 @@ namespace nnchip
 #pragma unroll
 			for (int i = 0; i < T; ++i) m_off[i] = -INFINITY, l[i] = 0.0f;
 
-			// The keys any pair of the launch attends to, within the split.
-			int kmin, kmax, unused;
-			attn_span(p.causal, p.window, p.pos0, p.n_seq, kmin, unused);
-			attn_span(p.causal, p.window, p.pos0 + p.n_tok - 1, p.n_seq, unused, kmax);
-			const int k0 = p.split_base + split * p.split_keys;
-			const int g_first = (kmin > k0 ? kmin : k0) / kQ4Rows;
-			const int g_last = (kmax < k0 + p.split_keys - 1 ? kmax : k0 + p.split_keys - 1) / kQ4Rows;
-			const int row_groups = p.rows / kQ4Rows, blocks = p.kv_dim / kQ4Block;
-			const unsigned char* recs = static_cast<const unsigned char*>(p.K) + static_cast<size_t>(kvh) * NB * kQ4Record;
-			const size_t group_bytes = static_cast<size_t>(blocks) * kQ4Record;
-			// (wavefront w takes the groups whose number in the split is w modulo kW)
-			int kg = k0 / kQ4Rows + wave;
-			if (kg < g_first) kg += (g_first - kg + kW - 1) / kW * kW;
-
-			// Up to 8 blocks the next group's records are in flight during the work on
-			// this one; 16 blocks' registers do not fit twice, and they are loaded here.
-			constexpr bool kAhead = NB <= 8;
-			auto records_of = [&](int n, record* r)
-			{
-#pragma unroll
-				for (int b = 0; b < NB; ++b)
-					r[b] = load_record(recs + static_cast<size_t>(n % row_groups) * group_bytes + b * kQ4Record, lane);
-			};
-			record r[NB];
-			if (kAhead && kg <= g_last) records_of(kg, r);
 			for (; kg <= g_last; kg += kW)
 			{
 				record nx[kAhead ? NB : 1];
@@ -271,10 +278,80 @@ namespace nnchip
 					else
 					{
 						const size_t at = (static_cast<size_t>(tok) * p.n_head + kvh * group + h) * HD + d;
-						p.out[at] = gated(acc * (sum > 0.0f ? 1.0f / sum : 0.0f), p.gate, at);
+						p.out[at] = gated(acc * (sum == 0.0f ? 0.0f : 1.0f / sum), p.gate, at);
 					}
 				}
 			}
+		}
+
+		// The ordered merge of a pair's splits: M = the largest offset, o and l summed
+		// relative to it. A work-group per (token, query head): every split's offset
+		// and sum in one load per thread, outputs in float4 columns times slices of
+		// the splits, joined in slice order. A split's thread and slice follow its
+		// absolute number (keys / split_keys), so a batch whose first split lies
+		// before a token's own gives the token the same sums (those splits add
+		// exact zeros).
+		constexpr int kMergeThreads = 256, kMergeAhead = 8;
+		static_assert(kDecodeMaxSplits == kMergeThreads, "a thread per split");
+		__global__ __launch_bounds__(kMergeThreads) void merge_q4_kernel(const decode_params p, int hd, int group)
+		{
+			__shared__ float s_f[kDecodeMaxSplits];
+			__shared__ float s_red[2][kMergeThreads / 64];
+			__shared__ float4 s_o[kMergeThreads];
+			const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+			const int qh = blockIdx.x, tok = blockIdx.y, kvh = qh / group, h = qh % group;
+			const int ns = p.n_split, cols = hd / 4, n_slices = kMergeThreads / cols;
+			const int c = tid % cols, slice = tid / cols;
+			const int base = p.split_base / p.split_keys; // the first split's number
+			const int mine = (tid - base) & (kDecodeMaxSplits - 1); // the thread's split
+			const int s0 = n_slices - 1 - (base + n_slices - 1 - slice) % n_slices; // the slice's first split
+			const float* part = p.part + ((static_cast<size_t>(tok) * p.n_kv + kvh) * ns * group + h) * (hd + 4);
+			const size_t step = static_cast<size_t>(group) * (hd + 4);
+
+			float m = -INFINITY, l = 0.0f;
+			if (mine < ns) m = part[mine * step + hd], l = part[mine * step + hd + 1];
+			float4 o[kMergeAhead]; // the slice's first splits, on their way meanwhile
+#pragma unroll
+			for (int i = 0; i < kMergeAhead; ++i)
+			{
+				const int s = s0 + i * n_slices;
+				o[i] = float4{0, 0, 0, 0};
+				if (slice < n_slices && s < ns) o[i] = *reinterpret_cast<const float4*>(part + s * step + 4 * c);
+			}
+			float mx = max_with_other_half(max_other_row(row_max(m)));
+			if (lane == 0) s_red[0][wave] = mx;
+			__syncthreads();
+			mx = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
+			const float f = fast_exp2(m - (mx == -INFINITY ? 0.0f : mx));
+			s_f[mine] = f;
+			l = wave_sum_dpp(l * f);
+			if (lane == 0) s_red[1][wave] = l;
+			__syncthreads();
+			float4 acc = {0, 0, 0, 0};
+			auto add = [&](const float4& v, float w)
+			{
+				acc.x = fmaf(v.x, w, acc.x);
+				acc.y = fmaf(v.y, w, acc.y);
+				acc.z = fmaf(v.z, w, acc.z);
+				acc.w = fmaf(v.w, w, acc.w);
+			};
+			if (slice < n_slices)
+			{
+#pragma unroll
+				for (int i = 0; i < kMergeAhead; ++i)
+					if (s0 + i * n_slices < ns) add(o[i], s_f[s0 + i * n_slices]);
+				for (int s = s0 + kMergeAhead * n_slices; s < ns; s += n_slices)
+					add(*reinterpret_cast<const float4*>(part + s * step + 4 * c), s_f[s]);
+			}
+			s_o[tid] = acc;
+			__syncthreads();
+			if (tid >= cols) return;
+			for (int i = 1; i < n_slices; ++i) add(s_o[i * cols + tid], 1.0f);
+			const float sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+			const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+			const size_t at = (static_cast<size_t>(tok) * p.n_head + qh) * hd + 4 * tid;
+			*reinterpret_cast<float4*>(p.out + at) = float4{gated(acc.x * inv, p.gate, at), gated(acc.y * inv, p.gate, at + 1),
+			                                                gated(acc.z * inv, p.gate, at + 2), gated(acc.w * inv, p.gate, at + 3)};
 		}
 
 		template <int NB>
@@ -294,7 +371,8 @@ namespace nnchip
 				run(std::integral_constant<int, kMost < 2 ? 1 : 2>());
 			else
 				run(std::integral_constant<int, kMost>());
-			if (p.n_split > 1) launch_merge_generic(p, n_tok, NB * kQ4Block, group, stream);
+			if (p.n_split > 1)
+				merge_q4_kernel<<<dim3(p.n_head, n_tok), kMergeThreads, 0, stream>>>(p, NB * kQ4Block, group);
 		}
 	}
 
