@@ -368,6 +368,7 @@ namespace nnchip
 			{
 				if constexpr (MODE == kQ4)
 				{
+					const q4_masks masks;
 #pragma unroll
 					for (int n = 0; n < G::NR; ++n)
 					{
@@ -377,10 +378,10 @@ namespace nnchip
 #pragma unroll
 						for (int t = 0; t < 2; ++t)
 						{
-							const f16x8 x = q4_k(t ? g.code[n].y : g.code[n].x, t ? g.ksz[n].y : g.ksz[n].x);
+							const f16x8 x = q4_k(t ? g.code[n].y : g.code[n].x, t ? g.ksz[n].y : g.ksz[n].x, masks);
 							*reinterpret_cast<f16x8*>(sk + (32 * gi + 16 * t + i) * G::KP + 32 * b + 8 * q) = x;
 							// (quarter q of the rows: rows 4 q + j and 16 + 4 q + j, i.e. s = q / 2, h = q % 2)
-							const f16x8 y = q4_v(t ? g.code[n].w : g.code[n].z, g.vs[n], g.vz[n]);
+							const f16x8 y = q4_v(t ? g.code[n].w : g.code[n].z, g.vs[n], g.vz[n], masks);
 							*reinterpret_cast<f16x8*>(sv + (32 * b + 16 * t + i) * G::VP + 32 * gi + 8 * q) = y;
 						}
 					}

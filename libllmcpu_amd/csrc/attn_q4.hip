@@ -78,12 +78,15 @@ namespace nnchip
 			return as_u32(is_lo ? l : h);
 		}
 
+		// Two wavefronts per SIMD where their registers fit (256 each).
+		constexpr int q4_per_simd(int nb, int t) { return nb <= 4 && nb * t <= 6 ? 2 : 1; }
+
 		template <int NB, int T>
-		__global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(1, 2))) void decode_q4_kernel(
+		__global__ __launch_bounds__(64 * kW, q4_per_simd(NB, T)) void decode_q4_kernel(
 			const decode_params p, int group)
 		{
 			constexpr int HD = NB * kQ4Block;
-			const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+			const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 			const int split = blockIdx.x, kvh = blockIdx.y;
 			const int c8 = lane & 7, g = lane >> 4;
 			const bool is_lo = (lane & 8) != 0;
@@ -105,20 +108,27 @@ namespace nnchip
 			int kg = k0 / kQ4Rows + wave;
 			if (kg < g_first) kg += (g_first - kg + kW - 1) / kW * kW;
 
-			// Up to 8 blocks the next group's records are in flight during the work on
-			// this one; 16 blocks' registers do not fit twice, and they are loaded here.
-			constexpr bool kAhead = NB <= 8;
-			auto records_of = [&](int n, record* r)
+			// Records in flight: kDepth - 1 groups ahead of the one worked on. (At 16
+			// blocks a group's registers do not fit twice.)
+			constexpr int kDepth = NB <= 4 && T == 1 ? 3 : NB <= 8 ? 2 : 1;
+			int row_group = kg % row_groups; // of the group loaded next
+			const int hop = kW % row_groups;
+			record r[kDepth][NB];
+			auto load_next = [&](record* to)
 			{
+				const unsigned char* at = recs + static_cast<size_t>(row_group) * group_bytes;
 #pragma unroll
-				for (int b = 0; b < NB; ++b)
-					r[b] = load_record(recs + static_cast<size_t>(n % row_groups) * group_bytes + b * kQ4Record, lane);
+				for (int b = 0; b < NB; ++b) to[b] = load_record(at + b * kQ4Record, lane);
+				row_group += hop;
+				if (row_group >= row_groups) row_group -= row_groups;
 			};
-			record r[NB];
-			if (kAhead && kg <= g_last) records_of(kg, r);
+#pragma unroll
+			for (int i = 0; i + 1 < kDepth; ++i)
+				if (kg + i * kW <= g_last) load_next(r[i]);
+
 			// Q: per pair brought under 2^15 by a power of two, then fp16 hi or lo.
 			f16x8 q[T][NB];
-			float back[T]; // 2^-that power, and log2(e) * scale
+			float back[T]; // 2^-that power, and log2(e) * |scale| (its sign is in q: a masked score stays the least)
 			int first[T], last[T];
 #pragma unroll
 			for (int i = 0; i < T; ++i)
@@ -144,13 +154,14 @@ namespace nnchip
 				m = column_max(m);
 				// (0, infinity and NaN: as they are)
 				const int e = m > 0.0f && m < INFINITY ? 14 - ilogbf(m) : 0;
-				back[i] = ldexpf(p.qscale, -e);
+				back[i] = fmaxf(ldexpf(fabsf(p.qscale), -e), 1.17549435e-38f);
+				const float sign = p.qscale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
 				for (int b = 0; b < NB; ++b)
 				{
 					u32x4 w;
 #pragma unroll
-					for (int j = 0; j < 4; ++j) w[j] = part_of(ldexpf(x[b][2 * j], e), ldexpf(x[b][2 * j + 1], e), is_lo);
+					for (int j = 0; j < 4; ++j) w[j] = part_of(sign * ldexpf(x[b][2 * j], e), sign * ldexpf(x[b][2 * j + 1], e), is_lo);
 					q[i][b] = as_f16x8(w);
 				}
 			}
@@ -160,21 +171,25 @@ namespace nnchip
 #pragma unroll
 			for (int i = 0; i < T; ++i) m_off[i] = -INFINITY, l[i] = 0.0f;
 
-			for (; kg <= g_last; kg += kW)
+			// Every pair of tile i sees the keys full_from[i] .. full_to[i].
+			int full_from[T], full_to[T];
+#pragma unroll
+			for (int i = 0; i < T; ++i)
 			{
-				record nx[kAhead ? NB : 1];
-				if constexpr (kAhead)
-					records_of(kg + kW <= g_last ? kg + kW : kg, nx);
-				else
-					records_of(kg, r);
-
+				const int a = (blockIdx.z * T + i) * 8, z = a + 7 < n_pairs ? a + 7 : n_pairs - 1;
+				attn_span(p.causal, p.window, p.pos0 + z / group, p.n_seq, full_from[i], unused);
+				attn_span(p.causal, p.window, p.pos0 + (a < n_pairs ? a : 0) / group, p.n_seq, unused, full_to[i]);
+			}
+			const q4_masks masks;
+			auto work = [&](const record* r)
+			{
 				f32x4 s[T][2] = {};
 #pragma unroll
 				for (int b = 0; b < NB; ++b)
 #pragma unroll
 					for (int t = 0; t < 2; ++t)
 					{
-						const f16x8 a = q4_k(t ? r[b].code.y : r[b].code.x, t ? r[b].ksz.y : r[b].ksz.x);
+						const f16x8 a = q4_k(t ? r[b].code.y : r[b].code.x, t ? r[b].ksz.y : r[b].ksz.x, masks);
 #pragma unroll
 						for (int i = 0; i < T; ++i) s[i][t] = mfma16x16x32(a, q[i][b], s[i][t]);
 					}
@@ -184,22 +199,32 @@ namespace nnchip
 				for (int i = 0; i < T; ++i)
 				{
 					float sc[8]; // tile t, row j: 4 t + j; key 32 kg + 16 t + 4 g + j
-					float m = -INFINITY;
 #pragma unroll
 					for (int j = 0; j < 8; ++j)
 					{
 						const float d = s[i][j >> 2][j & 3];
-						sc[j] = (d + ror8(d)) * back[i];
-						const int key = kg * kQ4Rows + 16 * (j >> 2) + 4 * g + (j & 3);
-						if (key < first[i] || key > last[i]) sc[j] = -INFINITY;
-						m = fmaxf(m, sc[j]);
+						sc[j] = d + ror8(d);
 					}
-					m = column_max(m);
-					const float was = m_off[i];
-					if (m > was + kRaise) // (the first keys of a span too: was is -inf)
+					if (kg * kQ4Rows < full_from[i] || kg * kQ4Rows + kQ4Rows - 1 > full_to[i])
 					{
-						m_off[i] = m - kBelow;
-						const float f = fast_exp2(was - m_off[i]);
+						asm volatile(""); // (a branch: most groups lie within every span)
+#pragma unroll
+						for (int j = 0; j < 8; ++j)
+						{
+							const int key = kg * kQ4Rows + 16 * (j >> 2) + 4 * g + (j & 3);
+							if (key < first[i] || key > last[i]) sc[j] = -INFINITY;
+						}
+					}
+					float m = sc[0];
+#pragma unroll
+					for (int j = 1; j < 8; ++j) m = fmaxf(m, sc[j]);
+					m = column_max(m) * back[i];
+					const bool up = m > m_off[i] + kRaise; // (the first keys of a span too: from -inf)
+					if (__any(up))
+					{
+						const float now = up ? m - kBelow : m_off[i];
+						const float f = up ? fast_exp2(m_off[i] - now) : 1.0f;
+						m_off[i] = now;
 						l[i] *= f;
 #pragma unroll
 						for (int b = 0; b < NB; ++b) o[i][b][0] *= f, o[i][b][1] *= f;
@@ -208,7 +233,7 @@ namespace nnchip
 #pragma unroll
 					for (int j = 0; j < 8; ++j)
 					{
-						sc[j] = fast_exp2(sc[j] - off);
+						sc[j] = fast_exp2(fmaf(sc[j], back[i], -off));
 						l[i] += sc[j];
 					}
 					u32x4 f;
@@ -222,13 +247,21 @@ namespace nnchip
 #pragma unroll
 					for (int t = 0; t < 2; ++t)
 					{
-						const f16x8 a = q4_v(t ? r[b].code.w : r[b].code.z, r[b].vs, r[b].vz);
+						const f16x8 a = q4_v(t ? r[b].code.w : r[b].code.z, r[b].vs, r[b].vz, masks);
 #pragma unroll
 						for (int i = 0; i < T; ++i) o[i][b][t] = mfma16x16x32(a, w[i], o[i][b][t]);
 					}
-				if constexpr (kAhead)
+			};
+			for (; kg <= g_last;)
+			{
 #pragma unroll
-					for (int b = 0; b < NB; ++b) r[b] = nx[b];
+				for (int i = 0; i < kDepth; ++i)
+				{
+					if (kg > g_last) break;
+					if (kDepth == 1 || kg + (kDepth - 1) * kW <= g_last) load_next(r[(i + kDepth - 1) % kDepth]);
+					work(r[i]);
+					kg += kW;
+				}
 			}
 
 			// The wavefronts' parts of each tile, joined in wavefront order.

@@ -57,24 +57,30 @@ namespace nnchip
 	// operations for eight codes with the fused multiply-adds that follow (a
 	// shift, four and-ors, four to remove the 1024, four to scale), where a
 	// conversion per code takes 24.
-	__device__ __forceinline__ void q4_codes(uint32_t w, f16x2 c[4])
+	// (The and and the or are one instruction if neither constant is a literal:
+	// q4_masks holds them in registers.)
+	struct q4_masks
 	{
-		const uint32_t k1024 = 0x64006400u;
+		uint32_t low = 0x000f000fu, high = 0x00f000f0u, k1024 = 0x64006400u;
+		__device__ __forceinline__ q4_masks() { asm("" : "+s"(low), "+s"(high), "+v"(k1024)); }
+	};
+	__device__ __forceinline__ void q4_codes(uint32_t w, const q4_masks& k, f16x2 c[4])
+	{
 		const uint32_t h = w >> 8;
 		const f16x2 m1024 = {static_cast<_Float16>(-1024.0f), static_cast<_Float16>(-1024.0f)};
 		const f16x2 m64 = {static_cast<_Float16>(-64.0f), static_cast<_Float16>(-64.0f)};
 		const f16x2 s16 = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
-		c[0] = as_f16x2((w & 0x000f000fu) | k1024) + m1024;
-		c[1] = __builtin_elementwise_fma(as_f16x2((w & 0x00f000f0u) | k1024), s16, m64);
-		c[2] = as_f16x2((h & 0x000f000fu) | k1024) + m1024;
-		c[3] = __builtin_elementwise_fma(as_f16x2((h & 0x00f000f0u) | k1024), s16, m64);
+		c[0] = as_f16x2((w & k.low) | k.k1024) + m1024;
+		c[1] = __builtin_elementwise_fma(as_f16x2((w & k.high) | k.k1024), s16, m64);
+		c[2] = as_f16x2((h & k.low) | k.k1024) + m1024;
+		c[3] = __builtin_elementwise_fma(as_f16x2((h & k.high) | k.k1024), s16, m64);
 	}
 
 	// A K word's values: sz holds the row's (s, z).
-	__device__ __forceinline__ f16x8 q4_k(uint32_t w, uint32_t sz)
+	__device__ __forceinline__ f16x8 q4_k(uint32_t w, uint32_t sz, const q4_masks& k)
 	{
 		f16x2 c[4];
-		q4_codes(w, c);
+		q4_codes(w, k, c);
 		const f16x2 h = as_f16x2(sz);
 		const f16x2 s = {h.x, h.x}, z = {h.y, h.y};
 		u32x4 r;
@@ -84,10 +90,10 @@ namespace nnchip
 	}
 
 	// A V word's values: s and z of its eight rows.
-	__device__ __forceinline__ f16x8 q4_v(uint32_t w, const u32x4& s, const u32x4& z)
+	__device__ __forceinline__ f16x8 q4_v(uint32_t w, const u32x4& s, const u32x4& z, const q4_masks& k)
 	{
 		f16x2 c[4];
-		q4_codes(w, c);
+		q4_codes(w, k, c);
 		u32x4 r;
 #pragma unroll
 		for (int j = 0; j < 4; ++j) r[j] = as_u32(__builtin_elementwise_fma(c[j], as_f16x2(s[j]), as_f16x2(z[j])));

@@ -185,6 +185,7 @@ namespace nnchip
 			const u32x4 vs = *reinterpret_cast<const u32x4*>(rec + kQ4VScales + 32 * g);
 			const u32x4 vz = *reinterpret_cast<const u32x4*>(rec + kQ4VScales + 32 * g + 16);
 			const int first = group * kQ4Rows - row0; // the group's first row, in the output
+			const q4_masks masks;
 			if constexpr (!RAW)
 			{
 				if (k_out)
@@ -192,7 +193,7 @@ namespace nnchip
 					for (int t = 0; t < 2; ++t)
 					{
 						const int r = first + 16 * t + i;
-						const f16x8 x = q4_k(t ? w.y : w.x, t ? ksz.y : ksz.x);
+						const f16x8 x = q4_k(t ? w.y : w.x, t ? ksz.y : ksz.x, masks);
 						if (r < 0 || r >= n_rows) continue;
 						float4* dst = reinterpret_cast<float4*>(static_cast<float*>(k_out) + static_cast<size_t>(r) * kv_dim +
 						                                        blk * kQ4Block + 8 * g);
@@ -204,7 +205,7 @@ namespace nnchip
 #pragma unroll
 					for (int t = 0; t < 2; ++t)
 					{
-						const f16x8 x = q4_v(t ? w.w : w.z, vs, vz);
+						const f16x8 x = q4_v(t ? w.w : w.z, vs, vz, masks);
 						float* dst = static_cast<float*>(v_out) + blk * kQ4Block + 16 * t + i;
 #pragma unroll
 						for (int n = 0; n < 8; ++n)
