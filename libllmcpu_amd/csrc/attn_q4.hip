@@ -81,6 +81,23 @@ namespace nnchip
 		// Two wavefronts per SIMD where their registers fit (256 each).
 		constexpr int q4_per_simd(int nb, int t) { return nb <= 4 && nb * t <= 6 ? 2 : 1; }
 
+		__device__ __forceinline__ void add_scaled(float4& acc, const float4& v, float w)
+		{
+			acc.x = fmaf(v.x, w, acc.x);
+			acc.y = fmaf(v.y, w, acc.y);
+			acc.z = fmaf(v.z, w, acc.z);
+			acc.w = fmaf(v.w, w, acc.w);
+		}
+
+		// Four outputs at element `at`: sums over their weights' sum.
+		__device__ __forceinline__ void write_out(const decode_params& p, size_t at, const float4& acc, float sum)
+		{
+			const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+			float4 y = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+			if (p.gate) y = float4{gated(y.x, p.gate, at), gated(y.y, p.gate, at + 1), gated(y.z, p.gate, at + 2), gated(y.w, p.gate, at + 3)};
+			*reinterpret_cast<float4*>(p.out + at) = y;
+		}
+
 		template <int NB, int T>
 		__global__ __launch_bounds__(64 * kW, q4_per_simd(NB, T)) void decode_q4_kernel(
 			const decode_params p, int group)
@@ -153,15 +170,16 @@ namespace nnchip
 				}
 				m = column_max(m);
 				// (0, infinity and NaN: as they are)
-				const int e = m > 0.0f && m < INFINITY ? 14 - ilogbf(m) : 0;
+				int e = m > 0.0f && m < INFINITY ? 14 - ilogbf(m) : 0;
+				e = e < 126 ? e : 126;
 				back[i] = fmaxf(ldexpf(fabsf(p.qscale), -e), 1.17549435e-38f);
-				const float sign = p.qscale < 0.0f ? -1.0f : 1.0f;
+				const float up = ldexpf(p.qscale < 0.0f ? -1.0f : 1.0f, e);
 #pragma unroll
 				for (int b = 0; b < NB; ++b)
 				{
 					u32x4 w;
 #pragma unroll
-					for (int j = 0; j < 4; ++j) w[j] = part_of(sign * ldexpf(x[b][2 * j], e), sign * ldexpf(x[b][2 * j + 1], e), is_lo);
+					for (int j = 0; j < 4; ++j) w[j] = part_of(x[b][2 * j] * up, x[b][2 * j + 1] * up, is_lo);
 					q[i][b] = as_f16x8(w);
 				}
 			}
@@ -284,35 +302,33 @@ namespace nnchip
 					}
 				if (lane < 8) s_o[wave][c8][HD] = m_off[i], s_o[wave][c8][HD + 1] = l[i];
 				__syncthreads();
-				for (int x = threadIdx.x; x < 8 * HD; x += 64 * kW)
+				const int pair0 = (blockIdx.z * T + i) * 8;
+				const int n_here = n_pairs - pair0 < 8 ? n_pairs - pair0 : 8;
+				for (int x = threadIdx.x; x < n_here * (HD / 4); x += 64 * kW) // a float4 of a pair
 				{
-					const int c = x / HD, d = x % HD;
-					const int pair = (blockIdx.z * T + i) * 8 + c;
-					if (pair >= n_pairs) break;
+					const int c = x / (HD / 4), d = 4 * (x % (HD / 4)), pair = pair0 + c;
+					const int tok = p.n_tok == 1 ? 0 : pair / group, h = pair - tok * group;
 					float mx = s_o[0][c][HD];
 #pragma unroll
 					for (int v = 1; v < kW; ++v) mx = fmaxf(mx, s_o[v][c][HD]);
 					const float off = mx == -INFINITY ? 0.0f : mx;
-					float acc = 0.0f, sum = 0.0f;
+					float4 acc = {0, 0, 0, 0};
+					float sum = 0.0f;
 #pragma unroll
 					for (int v = 0; v < kW; ++v)
 					{
 						const float f = fast_exp2(s_o[v][c][HD] - off);
-						acc = fmaf(s_o[v][c][d], f, acc);
+						add_scaled(acc, *reinterpret_cast<const float4*>(&s_o[v][c][d]), f);
 						sum = fmaf(s_o[v][c][HD + 1], f, sum);
 					}
-					const int tok = pair / group, h = pair % group;
 					if (p.n_split > 1)
 					{
 						float* dst = p.part + (((static_cast<size_t>(tok) * p.n_kv + kvh) * p.n_split + split) * group + h) * (HD + 4);
-						dst[d] = acc;
-						if (d == 0) dst[HD] = mx, dst[HD + 1] = sum;
+						*reinterpret_cast<float4*>(dst + d) = acc;
+						if (d == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(mx, sum);
 					}
 					else
-					{
-						const size_t at = (static_cast<size_t>(tok) * p.n_head + kvh * group + h) * HD + d;
-						p.out[at] = gated(acc * (sum == 0.0f ? 0.0f : 1.0f / sum), p.gate, at);
-					}
+						write_out(p, (static_cast<size_t>(tok) * p.n_head + kvh * group + h) * HD + d, acc, sum);
 				}
 			}
 		}
@@ -361,30 +377,20 @@ namespace nnchip
 			if (lane == 0) s_red[1][wave] = l;
 			__syncthreads();
 			float4 acc = {0, 0, 0, 0};
-			auto add = [&](const float4& v, float w)
-			{
-				acc.x = fmaf(v.x, w, acc.x);
-				acc.y = fmaf(v.y, w, acc.y);
-				acc.z = fmaf(v.z, w, acc.z);
-				acc.w = fmaf(v.w, w, acc.w);
-			};
 			if (slice < n_slices)
 			{
 #pragma unroll
 				for (int i = 0; i < kMergeAhead; ++i)
-					if (s0 + i * n_slices < ns) add(o[i], s_f[s0 + i * n_slices]);
+					if (s0 + i * n_slices < ns) add_scaled(acc, o[i], s_f[s0 + i * n_slices]);
 				for (int s = s0 + kMergeAhead * n_slices; s < ns; s += n_slices)
-					add(*reinterpret_cast<const float4*>(part + s * step + 4 * c), s_f[s]);
+					add_scaled(acc, *reinterpret_cast<const float4*>(part + s * step + 4 * c), s_f[s]);
 			}
 			s_o[tid] = acc;
 			__syncthreads();
 			if (tid >= cols) return;
-			for (int i = 1; i < n_slices; ++i) add(s_o[i * cols + tid], 1.0f);
+			for (int i = 1; i < n_slices; ++i) add_scaled(acc, s_o[i * cols + tid], 1.0f);
 			const float sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
-			const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-			const size_t at = (static_cast<size_t>(tok) * p.n_head + qh) * hd + 4 * tid;
-			*reinterpret_cast<float4*>(p.out + at) = float4{gated(acc.x * inv, p.gate, at), gated(acc.y * inv, p.gate, at + 1),
-			                                                gated(acc.z * inv, p.gate, at + 2), gated(acc.w * inv, p.gate, at + 3)};
+			write_out(p, (static_cast<size_t>(tok) * p.n_head + qh) * hd + 4 * tid, acc, sum);
 		}
 
 		template <int NB>
