@@ -56,7 +56,7 @@ namespace nnchip
 			static constexpr int NK = KS * HD / 8 / 256; // 8-element pieces of K per thread
 			static constexpr int NV = (HD / 2 * (KS / 8) + 255) / 256; // (column pair, 8 keys) pieces of V per thread
 			static constexpr int NR = (KS / 32 * (HD / 32) + kWaves - 1) / kWaves; // records per wavefront
-			static constexpr int PER_SIMD = HD <= (MODE == kBf16 ? 128 : 64) ? 2 : 1; // wavefronts
+			static constexpr int PER_SIMD = HD <= 128 ? 2 : 1; // wavefronts
 		};
 
 		// What a step's loads leave in registers until LDS is free.
