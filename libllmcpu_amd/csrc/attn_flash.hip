@@ -3,14 +3,18 @@
 // and batches over the 4-bit cache (kv_q4.h).
 //
 // The rows of a KV head are (token, query head) pairs, token by token, so the
-// heads that share its keys share every load. A work-group of four wavefronts
-// owns 128 rows of one sequence and walks their keys in steps: the step's K, and
-// V transposed, go to LDS once for all rows, and each wavefront computes for its
-// 32 rows
-//   S^T = K Q^T        (a lane holds 16 keys' scores of one row per 32 x 32 tile)
+// heads that share its keys share every load. A work-group of RG x KG wavefronts
+// owns RG row groups of TR rows of one sequence and walks their keys in steps,
+// every KG-th step a key group's. A step's K, and V transposed, go to LDS once
+// for all row groups, and each wavefront computes for its TR rows
+//   S^T = K Q^T        (a lane holds several keys' scores of one row)
 //   P = 2^(S - offset) (running offset and sum per row; see kRaise)
 //   O^T += V^T P^T     (the lane's own weights are the operand: a lane's eight k
 //                       slots of a product are taken to be the keys it holds)
+// The key groups of a row meet in LDS at the end. TR is 32 (32 x 32 products) up
+// to head_dim 128, and 16 (16 x 16 products, half the rows' O and Q) at 256, so
+// that two wavefronts' registers fit on a SIMD: one's products run beside the
+// other's softmax and conversions.
 // One pass over the keys; only steps that cross a row's span are masked.
 //
 // Precision. BF16: the operands are exact, P is rounded to BF16 (2^-9 of a
@@ -35,7 +39,6 @@ namespace nnchip
 	namespace
 	{
 		constexpr int kBf16 = 0, kF32 = 1, kQ4 = 2;
-		constexpr int kWaves = 4, kRows = 32 * kWaves;
 		// Weights are 2^(score - offset); the offset is raised, to kBelow under the
 		// largest score so far, when a score passes it by more than kRaise: weights
 		// stay in fp16's range, and rescaling O is rare.
@@ -43,36 +46,40 @@ namespace nnchip
 
 		constexpr int kBufferFlags = 0x00020000; // buffer descriptor word 3: raw 32-bit data
 
-		template <int MODE, int HD>
+		template <int MODE_, int HD_, int TR_, int RG_, int KG_>
 		struct shape
 		{
-			static constexpr int KS = HD <= 128 ? 64 : 32; // keys of a step
-			static constexpr int KT = KS / 32; // 32-key tiles
+			static constexpr int MODE = MODE_, HD = HD_, TR = TR_, RG = RG_, KG = KG_;
+			static constexpr int WAVES = RG * KG, ROWS = TR * RG;
+			static constexpr int KS = HD <= (MODE == kF32 ? 96 : 128) ? 64 : 32; // keys of a step
 			static constexpr int KP = HD + 8, VP = KS + 8; // halves per K row, per V^T row (an odd number of 16 bytes)
 			static constexpr int PARTS = MODE == kF32 ? 2 : 1; // hi, lo
 			static constexpr int K_HALVES = KS * KP, V_HALVES = HD * VP;
-			static constexpr int TILE_BYTES = 2 * PARTS * (K_HALVES + V_HALVES);
-			static constexpr int BYTES = TILE_BYTES;
-			static constexpr int NK = KS * HD / 8 / 256; // 8-element pieces of K per thread
-			static constexpr int NV = (HD / 2 * (KS / 8) + 255) / 256; // (column pair, 8 keys) pieces of V per thread
-			static constexpr int NR = (KS / 32 * (HD / 32) + kWaves - 1) / kWaves; // records per wavefront
-			static constexpr int PER_SIMD = HD <= 128 ? 2 : 1; // wavefronts
+			static constexpr int TILE_BYTES = 2 * PARTS * (K_HALVES + V_HALVES); // of a key group
+			static constexpr int MEET_BYTES = (KG - 1) * RG * (TR * HD + 128) * 4;
+			static constexpr int BYTES = KG * TILE_BYTES > MEET_BYTES ? KG * TILE_BYTES : MEET_BYTES;
+			static constexpr int THREADS = 64 * RG; // of a key group
+			static constexpr int NK = KS * HD / 8 / THREADS; // 8-element pieces of K per thread
+			static constexpr int NV = (HD / 2 * (KS / 8) + THREADS - 1) / THREADS; // (column pair, 8 keys) pieces of V per thread
+			static constexpr int NR = (KS / 32 * (HD / 32) + RG - 1) / RG; // records per wavefront
+			static constexpr int NS = KS / TR, NO = HD / TR, EL = TR * TR / 64; // score tiles, output tiles, registers of one
+			static constexpr int QD = 512 / TR, NQ = HD / QD; // columns of a product, products over head_dim
+						static_assert(NK * THREADS * 8 == KS * HD && BYTES <= 160 << 10, "shape");
 		};
 
 		// What a step's loads leave in registers until LDS is free.
-		template <int MODE, int HD>
+		template <class G, bool Q4>
 		struct step_regs
 		{
-			u32x4 k[shape<MODE, HD>::NK * shape<MODE, HD>::PARTS];
-			uint32_t v[shape<MODE, HD>::NV][8 * shape<MODE, HD>::PARTS];
+			u32x4 k[G::NK * G::PARTS];
+			uint32_t v[G::NV][8 * G::PARTS];
 		};
-		// (4-bit: the wavefront's records)
-		template <int HD>
-		struct step_regs<kQ4, HD>
+		template <class G>
+		struct step_regs<G, true> // (4-bit: the wavefront's records)
 		{
-			u32x4 code[shape<kQ4, HD>::NR];
-			u32x2 ksz[shape<kQ4, HD>::NR];
-			u32x4 vs[shape<kQ4, HD>::NR], vz[shape<kQ4, HD>::NR];
+			u32x4 code[G::NR];
+			u32x2 ksz[G::NR];
+			u32x4 vs[G::NR], vz[G::NR];
 		};
 
 		__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
@@ -168,20 +175,52 @@ namespace nnchip
 			}
 		}
 
-		template <int MODE, int HD, int NSEQ>
-		__global__ __launch_bounds__(64 * kWaves, (shape<MODE, HD>::PER_SIMD)) void flash_kernel(const flash_params p,
-		                                                                                      const flash_seqs<NSEQ> seqs)
+		__device__ __forceinline__ f32x4 mfma(const bf16x8& a, const bf16x8& b, const f32x4& c) { return mfma16x16x32(a, b, c); }
+		__device__ __forceinline__ f32x4 mfma(const f16x8& a, const f16x8& b, const f32x4& c) { return mfma16x16x32(a, b, c); }
+		__device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) { return mfma32x32x16(a, b, c); }
+		__device__ __forceinline__ f32x16 mfma(const f16x8& a, const f16x8& b, const f32x16& c) { return mfma32x32x16(a, b, c); }
+
+		// Over the lanes that hold the same row.
+		template <int TR>
+		__device__ __forceinline__ float row_max(float x)
 		{
-			using G = shape<MODE, HD>;
-			constexpr int KS = G::KS, KT = G::KT;
+			if constexpr (TR == 16)
+			{
+				const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+				x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+			}
+			return max_with_other_half(x);
+		}
+		template <int TR>
+		__device__ __forceinline__ float row_sum(float x)
+		{
+			return add_with_other_half(TR == 16 ? add_with_other_row(x) : x);
+		}
+
+		template <class G, int NSEQ>
+		__global__ __launch_bounds__(64 * G::WAVES, 2) void flash_kernel(const flash_params p, const flash_seqs<NSEQ> seqs)
+		{
+			constexpr int MODE = G::MODE, HD = G::HD, TR = G::TR, KS = G::KS, NS = G::NS, NO = G::NO, EL = G::EL;
 			constexpr bool SPLIT = MODE != kBf16; // Q and P as hi + lo
 			typedef std::conditional_t<MODE == kBf16, bf16x8, f16x8> op8;
+			typedef std::conditional_t<TR == 32, f32x16, f32x4> acc_t;
+			typedef step_regs<G, MODE == kQ4> regs_t;
 			__shared__ __align__(16) unsigned char smem[G::BYTES];
-			__shared__ uint32_t s_max[2][kWaves];
-			uint16_t* const sk = reinterpret_cast<uint16_t*>(smem);
-			uint16_t* const sv = sk + G::PARTS * G::K_HALVES;
+			__shared__ uint32_t s_max[2][G::WAVES];
+			__shared__ uint32_t s_bad;
 
-			const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r32 = lane & 31, half = lane >> 5;
+			const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+			const int rg = wave % G::RG, kg = wave / G::RG; // row group, key group
+			const int kt_id = threadIdx.x - 64 * G::RG * kg; // thread of the key group
+			const int col = lane % TR, sub = lane / TR; // the lane's row of the row group, its share of a row's keys
+			uint16_t* const sk = reinterpret_cast<uint16_t*>(smem + kg * G::TILE_BYTES);
+			uint16_t* const sv = sk + G::PARTS * G::K_HALVES;
+			if constexpr (MODE != kQ4)
+			{
+				if (threadIdx.x == 0) s_bad = 0;
+				__syncthreads();
+			}
+
 			const int hd = p.head_dim, group = p.n_head / p.n_kv;
 			const int kvh = static_cast<int>(blockIdx.x % p.n_kv), tile = static_cast<int>(blockIdx.x / p.n_kv);
 
@@ -199,28 +238,27 @@ namespace nnchip
 			const size_t row_at = static_cast<size_t>(seqs.start[s_idx]); // of the sequence's first token
 			const long long n_rows = static_cast<long long>(len) * group;
 			// (the last rows of a causal sequence have the most keys: they go first)
-			const int n_blk = static_cast<int>((n_rows + kRows - 1) / kRows);
-			const long long r0 = static_cast<long long>(n_blk - 1 - (tile - seqs.tile[s_idx])) * kRows;
+			const int n_blk = static_cast<int>((n_rows + G::ROWS - 1) / G::ROWS);
+			const long long r0 = static_cast<long long>(n_blk - 1 - (tile - seqs.tile[s_idx])) * G::ROWS;
 			const int pos0 = MODE == kQ4 ? p.pos0 : 0, n_keys = MODE == kQ4 ? p.n_seq : len;
 
 			auto token_of = [&](long long r) { return static_cast<int>((r < n_rows ? r : n_rows - 1) / group); };
 			auto span_of = [&](long long r, int& a, int& b) { attn_span(p.causal, p.window, pos0 + token_of(r), n_keys, a, b); };
 
 			// The lane's row, and the keys of the work-group's and the wavefront's rows.
-			const long long row = r0 + 32 * wave + r32;
+			const long long w0 = r0 + TR * rg, row = w0 + col;
 			const bool real = row < n_rows;
 			const int tok = token_of(row), head = kvh * group + (real ? static_cast<int>(row % group) : 0);
 			int first, last;
 			attn_span(p.causal, p.window, pos0 + tok, n_keys, first, last);
-			int kmin, kmax, wmin, wmax, full_from, full_to, unused;
+			int kmin, kmax, full_from, full_to, unused;
 			span_of(r0, kmin, unused);
-			span_of(r0 + kRows - 1, unused, kmax);
-			span_of(r0 + 32 * wave, wmin, full_to); // every row of the wavefront sees full_from .. full_to
-			span_of(r0 + 32 * wave + 31, full_from, wmax);
-			const bool wave_real = r0 + 32 * wave < n_rows;
+			span_of(r0 + G::ROWS - 1, unused, kmax);
+			span_of(w0, unused, full_to); // every row of the wavefront sees full_from .. full_to
+			span_of(w0 + TR - 1, full_from, unused);
 
 			// ---- Q ----
-			constexpr int NQ = HD / 16;
+			constexpr int NQ = G::NQ;
 			op8 qh[NQ];
 			f16x8 ql[SPLIT ? NQ : 1];
 			// (S * sc in log2 units; the scale's sign goes into Q, so that a masked
@@ -233,7 +271,7 @@ namespace nnchip
 #pragma unroll
 				for (int ks = 0; ks < NQ; ++ks)
 				{
-					const int d = 16 * ks + 8 * half;
+					const int d = G::QD * ks + 8 * sub;
 					u32x4 w = {0, 0, 0, 0};
 					if (d < hd) w = *reinterpret_cast<const u32x4*>(q + d) ^ u32x4{flip, flip, flip, flip};
 					qh[ks] = as_bf16x8(w);
@@ -247,7 +285,7 @@ namespace nnchip
 #pragma unroll
 				for (int ks = 0; ks < NQ; ++ks)
 				{
-					const int d = 16 * ks + 8 * half;
+					const int d = G::QD * ks + 8 * sub;
 					float4 u = {0, 0, 0, 0}, v = {0, 0, 0, 0};
 					if (d < hd) u = *reinterpret_cast<const float4*>(q + d), v = *reinterpret_cast<const float4*>(q + d + 4);
 					if constexpr (MODE == kQ4) // (the k slot order of the 4-bit values)
@@ -259,7 +297,7 @@ namespace nnchip
 #pragma unroll
 					for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[ks][j]));
 				}
-				m = max_with_other_half(m);
+				m = row_max<TR>(m);
 				// (0, infinity and NaN: as they are)
 				const int e = m > 0.0f && m < INFINITY ? up_to_2_15(__float_as_uint(m)) : 0;
 				const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
@@ -287,8 +325,9 @@ namespace nnchip
 			// step (columns past head_dim: an offset past any descriptor).
 			constexpr int ESIZE = MODE == kBf16 ? 2 : 4;
 			const int blocks = hd / kQ4Block; // 4-bit: records of a KV head and group
-			// Key u of a V piece: set (tile, s, h), k slot order (keys 8 s + 4 h + j and
-			// 16 + 8 s + 4 h + j alternate).
+			// V^T's rows hold 32 keys as four pieces of eight k slots: keys 4 x + j and
+			// 16 + 4 x + j alternate in piece x, which are keys whose weights one lane
+			// holds, in either product's layout.
 			constexpr uint32_t kNowhere = 0x80000000u;
 			uint32_t k_off[G::NK], v_off[G::NV];
 			if constexpr (MODE != kQ4)
@@ -296,25 +335,26 @@ namespace nnchip
 #pragma unroll
 				for (int n = 0; n < G::NK; ++n)
 				{
-					const int c = threadIdx.x + 256 * n, d = 8 * (c % (HD / 8));
+					const int c = kt_id + G::THREADS * n, d = 8 * (c % (HD / 8));
 					k_off[n] = d < hd ? static_cast<uint32_t>((c / (HD / 8)) * p.k_stride + d) * ESIZE : kNowhere;
 				}
 #pragma unroll
 				for (int n = 0; n < G::NV; ++n)
 				{
-					const int c = threadIdx.x + 256 * n, set = c / (HD / 2), d = 2 * (c % (HD / 2));
-					const int key = 32 * (set >> 2) + 8 * ((set >> 1) & 1) + 4 * (set & 1);
+					const int c = kt_id + G::THREADS * n, set = c / (HD / 2), d = 2 * (c % (HD / 2));
+					const int key = 32 * (set >> 2) + 4 * (set & 3);
 					v_off[n] = set < KS / 8 && d < hd ? static_cast<uint32_t>(key * p.v_stride + d) * ESIZE : kNowhere;
 				}
 			}
-			// Rows k0 .. of a tensor (at most KS of them, as far as the sequence goes).
+			// Rows k0 .. of a tensor (at most KS of them, as far as the sequence goes; past
+			// the work-group's last key none: zeros).
 			auto rows_from = [&](const void* base, size_t stride, int k0)
 			{
-				const int n = n_keys - k0 < KS ? n_keys - k0 : KS;
+				const int n = k0 > kmax ? 0 : n_keys - k0 < KS ? n_keys - k0 : KS;
 				const char* at = static_cast<const char*>(base) + ((row_at + k0) * stride + static_cast<size_t>(kvh) * hd) * ESIZE;
-				return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, static_cast<int>(((n - 1) * stride + hd) * ESIZE), kBufferFlags);
+				return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, n ? static_cast<int>(((n - 1) * stride + hd) * ESIZE) : 0, kBufferFlags);
 			};
-			auto load_step = [&](int k0, step_regs<MODE, HD>& g)
+			auto load_step = [&](int k0, regs_t& g)
 			{
 				if constexpr (MODE == kQ4)
 				{
@@ -322,11 +362,11 @@ namespace nnchip
 #pragma unroll
 					for (int n = 0; n < G::NR; ++n)
 					{
-						const int rec = wave * G::NR + n, b = rec % (HD / 32), gi = rec / (HD / 32);
+						const int rec = rg * G::NR + n, b = rec % (HD / 32), gi = rec / (HD / 32);
 						g.code[n] = u32x4{0, 0, 0, 0};
 						g.ksz[n] = u32x2{0, 0};
 						g.vs[n] = g.vz[n] = u32x4{0, 0, 0, 0};
-						if (gi >= KT || b >= blocks || k0 + 32 * gi > kmax) continue;
+						if (gi >= KS / 32 || b >= blocks || k0 + 32 * gi > kmax) continue;
 						const unsigned char* at = static_cast<const unsigned char*>(p.k) +
 						                          (static_cast<size_t>((k0 / kQ4Rows + gi) % groups) * (p.n_kv * blocks) + kvh * blocks + b) * kQ4Record;
 						g.code[n] = *reinterpret_cast<const u32x4*>(at + 16 * lane);
@@ -364,7 +404,7 @@ namespace nnchip
 			};
 
 			// The registers' K rows and V^T rows into LDS (F32: times 2^ek, 2^ev).
-			auto store_step = [&](const step_regs<MODE, HD>& g, int ek, int ev)
+			auto store_step = [&](const regs_t& g, int ek, int ev)
 			{
 				if constexpr (MODE == kQ4)
 				{
@@ -372,15 +412,15 @@ namespace nnchip
 #pragma unroll
 					for (int n = 0; n < G::NR; ++n)
 					{
-						const int rec = wave * G::NR + n, b = rec % (HD / 32), gi = rec / (HD / 32);
-						if (gi >= KT) continue;
+						const int rec = rg * G::NR + n, b = rec % (HD / 32), gi = rec / (HD / 32);
+						if (gi >= KS / 32) continue;
 						const int i = lane & 15, q = lane >> 4;
 #pragma unroll
 						for (int t = 0; t < 2; ++t)
 						{
 							const f16x8 x = q4_k(t ? g.code[n].y : g.code[n].x, t ? g.ksz[n].y : g.ksz[n].x, masks);
 							*reinterpret_cast<f16x8*>(sk + (32 * gi + 16 * t + i) * G::KP + 32 * b + 8 * q) = x;
-							// (quarter q of the rows: rows 4 q + j and 16 + 4 q + j, i.e. s = q / 2, h = q % 2)
+							// (quarter q of the rows is V^T's piece q)
 							const f16x8 y = q4_v(t ? g.code[n].w : g.code[n].z, g.vs[n], g.vz[n], masks);
 							*reinterpret_cast<f16x8*>(sv + (32 * b + 16 * t + i) * G::VP + 32 * gi + 8 * q) = y;
 						}
@@ -391,13 +431,13 @@ namespace nnchip
 #pragma unroll
 					for (int n = 0; n < G::NK; ++n)
 					{
-						const int c = threadIdx.x + 256 * n;
+						const int c = kt_id + G::THREADS * n;
 						*reinterpret_cast<u32x4*>(sk + c / (HD / 8) * G::KP + 8 * (c % (HD / 8))) = g.k[n];
 					}
 #pragma unroll
 					for (int n = 0; n < G::NV; ++n)
 					{
-						const int c = threadIdx.x + 256 * n, set = c / (HD / 2), d = 2 * (c % (HD / 2));
+						const int c = kt_id + G::THREADS * n, set = c / (HD / 2), d = 2 * (c % (HD / 2));
 						if (set >= KS / 8) continue;
 						u32x4 a, b; // columns d and d + 1
 #pragma unroll
@@ -415,7 +455,7 @@ namespace nnchip
 #pragma unroll
 					for (int n = 0; n < G::NK; ++n)
 					{
-						const int c = threadIdx.x + 256 * n;
+						const int c = kt_id + G::THREADS * n;
 						u32x4 h, l;
 #pragma unroll
 						for (int j = 0; j < 4; ++j)
@@ -433,7 +473,7 @@ namespace nnchip
 #pragma unroll
 					for (int n = 0; n < G::NV; ++n)
 					{
-						const int c = threadIdx.x + 256 * n, set = c / (HD / 2), d = 2 * (c % (HD / 2));
+						const int c = kt_id + G::THREADS * n, set = c / (HD / 2), d = 2 * (c % (HD / 2));
 						if (set >= KS / 8) continue;
 #pragma unroll
 						for (int col = 0; col < 2; ++col)
@@ -456,34 +496,40 @@ namespace nnchip
 			};
 
 			// ---- the walk ----
-			f32x16 o[HD / 32] = {};
+			acc_t o[NO] = {};
 			float off = -INFINITY, l = 0.0f;
-			int ev = 1000; // F32: O is in units of 2^-ev (1000: nothing added yet)
-			// (raises the offset for a largest score m, in log2 units)
+			// F32: V goes to LDS times 2^ev, O is in units of 2^-ev_o (1000: nothing yet).
+			int ev = 1000, ev_o = 1000;
+			// Raises the offset for a largest score m (in log2 units), and takes O to ev's
+			// units.
 			auto raise = [&](float m)
 			{
 				const bool up = m > off + kRaise;
-				if (__any(up))
+				if (__any(up) || (MODE == kF32 && ev_o != ev))
 				{
 					const float now = up ? m - kBelow : off;
-					// (equal ones first: -inf - -inf is NaN)
-					const float f = now == off ? 1.0f : fast_exp2(off - now);
+					float f = up ? fast_exp2(off - now) : 1.0f; // (equal ones: -inf - -inf is NaN)
 					off = now;
 					l *= f;
+					if constexpr (MODE == kF32)
+					{
+						if (ev_o != 1000) f = ldexpf(f, ev - ev_o);
+						ev_o = ev;
+					}
 #pragma unroll
-					for (int dt = 0; dt < HD / 32; ++dt) o[dt] *= f;
+					for (int dt = 0; dt < NO; ++dt) o[dt] *= f;
 				}
 			};
 
-			bool by_vector = false;
-			step_regs<MODE, HD> regs;
+			regs_t regs;
 			const int k_first = kmin / KS * KS;
-			if (k_first <= kmax) load_step(k_first, regs);
-			for (int k0 = k_first; k0 <= kmax; k0 += KS)
+			const int n_steps = kmax < k_first ? 0 : (kmax - k_first) / KS + 1;
+			if (n_steps) load_step(k_first + kg * KS, regs);
+			for (int step = kg; step - kg < n_steps; step += G::KG) // (as often for every key group)
 			{
+				const int k0 = k_first + step * KS;
 				// Largest magnitudes (F32), or whether V holds an infinite or NaN element
 				// (BF16, masked steps).
-				bool slow = false;
 				int ek = 0;
 				if constexpr (MODE == kF32)
 				{
@@ -504,7 +550,7 @@ namespace nnchip
 				{
 					int a, b;
 					span_of(r0, unused, b);
-					span_of(r0 + kRows - 1, a, unused);
+					span_of(r0 + G::ROWS - 1, a, unused);
 					if (k0 < a || k0 + KS - 1 > b) // some row of the work-group does not see them all
 					{
 						bool bad = false;
@@ -513,9 +559,7 @@ namespace nnchip
 #pragma unroll
 							for (int u = 0; u < 8; ++u)
 								bad |= (regs.v[n][u] & 0x7f80u) == 0x7f80u || (regs.v[n][u] & 0x7f800000u) == 0x7f800000u;
-						if (lane == 0) s_max[0][wave] = 0;
-						if (__any(bad) && lane == 0) s_max[0][wave] = 1;
-						slow = true; // (to be looked at)
+						if (__any(bad)) s_bad = 1;
 					}
 				}
 				__syncthreads(); // every wavefront is done with the step before
@@ -523,115 +567,111 @@ namespace nnchip
 				{
 					uint32_t mk = 0, mv = 0;
 #pragma unroll
-					for (int w = 0; w < kWaves; ++w) mk = umax(mk, s_max[0][w]), mv = umax(mv, s_max[1][w]);
-					slow = mk >= 0x7f800000u || mv >= 0x7f800000u;
-					if (!slow)
+					for (int w = 0; w < G::RG; ++w) mk = umax(mk, s_max[0][kg * G::RG + w]), mv = umax(mv, s_max[1][kg * G::RG + w]);
+					mk = __builtin_amdgcn_readfirstlane(mk);
+					mv = __builtin_amdgcn_readfirstlane(mv);
+					if (mk >= 0x7f800000u || mv >= 0x7f800000u)
+						s_bad = 1; // (what this step computes is not used)
+					else
 					{
 						ek = up_to_2_15(mk);
 						const int want = mv == 0 ? ev : up_to_2_15(mv);
-						if (want < ev) // (V grows: O follows)
-						{
-							if (ev != 1000)
-#pragma unroll
-								for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-									for (int i = 0; i < 16; ++i) o[dt][i] = ldexpf(o[dt][i], want - ev);
-							ev = want;
-						}
+						if (want < ev) ev = want; // (V grows: O follows, in raise)
 					}
 				}
-				else if constexpr (MODE == kBf16)
-				{
-					if (slow) slow = (s_max[0][0] | s_max[0][1] | s_max[0][2] | s_max[0][3]) != 0;
-				}
-				if (MODE != kQ4 && __builtin_amdgcn_readfirstlane(slow))
-				{
-					by_vector = true; // (the whole work-group)
-					break;
-				}
-
+				// (a key group past the last step stores zeros, and all its keys are masked)
 				store_step(regs, ek, ev);
-				if (k0 + KS <= kmax) load_step(k0 + KS, regs);
+				if (step + G::KG - kg < n_steps) load_step(k0 + G::KG * KS, regs);
 				__syncthreads();
-				if (!wave_real || k0 > wmax || k0 + KS - 1 < wmin) continue;
 
-				f32x16 s[KT] = {};
+				acc_t s[NS] = {};
 #pragma unroll
-				for (int kt = 0; kt < KT; ++kt)
+				for (int t = 0; t < NS; ++t)
 #pragma unroll
 					for (int ks = 0; ks < NQ; ++ks)
 					{
-						const uint16_t* at = sk + (32 * kt + r32) * G::KP + 16 * ks + 8 * half;
+						const uint16_t* at = sk + (TR * t + col) * G::KP + G::QD * ks + 8 * sub;
 						const op8 a = *reinterpret_cast<const op8*>(at);
-						s[kt] = mfma32x32x16(a, qh[ks], s[kt]);
-						if constexpr (SPLIT) s[kt] = mfma32x32x16(a, ql[ks], s[kt]);
-						if constexpr (MODE == kF32) s[kt] = mfma32x32x16(*reinterpret_cast<const op8*>(at + G::K_HALVES), qh[ks], s[kt]);
+						s[t] = mfma(a, qh[ks], s[t]);
+						if constexpr (SPLIT) s[t] = mfma(a, ql[ks], s[t]);
+						if constexpr (MODE == kF32) s[t] = mfma(*reinterpret_cast<const op8*>(at + G::K_HALVES), qh[ks], s[t]);
 					}
 				float f = sc;
 				if constexpr (MODE == kF32) f = fminf(fmaxf(ldexpf(sc, -ek), 1.17549435e-38f), 1e36f);
 				if (k0 < full_from || k0 + KS - 1 > full_to)
 #pragma unroll
-					for (int kt = 0; kt < KT; ++kt)
+					for (int t = 0; t < NS; ++t)
 #pragma unroll
-						for (int i = 0; i < 16; ++i)
+						for (int i = 0; i < EL; ++i)
 						{
-							const int key = k0 + 32 * kt + 8 * (i >> 2) + 4 * half + (i & 3);
-							if (key < first || key > last) s[kt][i] = -INFINITY;
+							const int key = k0 + TR * t + 8 * (i >> 2) + 4 * sub + (i & 3);
+							if (key < first || key > last) s[t][i] = -INFINITY;
 						}
 				float m = s[0][0];
 #pragma unroll
-				for (int kt = 0; kt < KT; ++kt)
+				for (int t = 0; t < NS; ++t)
 #pragma unroll
-					for (int i = 0; i < 16; ++i) m = fmaxf(m, s[kt][i]);
-				raise(max_with_other_half(m) * f);
+					for (int i = 0; i < EL; ++i) m = fmaxf(m, s[t][i]);
+				raise(row_max<TR>(m) * f);
 				const float at = off == -INFINITY ? 0.0f : off;
 #pragma unroll
-				for (int kt = 0; kt < KT; ++kt)
+				for (int t = 0; t < NS; ++t)
 #pragma unroll
-					for (int i = 0; i < 16; ++i)
+					for (int i = 0; i < EL; ++i)
 					{
-						s[kt][i] = fast_exp2(fmaf(s[kt][i], f, -at));
-						l += s[kt][i];
+						s[t][i] = fast_exp2(fmaf(s[t][i], f, -at));
+						l += s[t][i];
 					}
+				// (a product's 64 * 8 / TR keys: half a 32-key tile's pieces, or all four)
 #pragma unroll
-				for (int kt = 0; kt < KT; ++kt)
+				for (int x = 0; x < KS * TR / 512; ++x)
+				{
+					u32x4 wh, wl;
 #pragma unroll
-					for (int h = 0; h < 2; ++h)
+					for (int j = 0; j < 4; ++j)
 					{
-						u32x4 wh, wl;
-#pragma unroll
-						for (int j = 0; j < 4; ++j)
+						float a, b;
+						if constexpr (TR == 32)
+							a = s[x >> 1][4 * (x & 1) + j], b = s[x >> 1][8 + 4 * (x & 1) + j];
+						else
+							a = s[2 * x][j], b = s[2 * x + 1][j];
+						if constexpr (SPLIT)
 						{
-							const float a = s[kt][4 * h + j], b = s[kt][8 + 4 * h + j];
-							if constexpr (SPLIT)
-							{
-								uint32_t x, y;
-								split_weights(a, b, x, y);
-								wh[j] = x;
-								wl[j] = y;
-							}
-							else
-								wh[j] = cvt_pk_bf16(a, b);
+							uint32_t y, z;
+							split_weights(a, b, y, z);
+							wh[j] = y;
+							wl[j] = z;
 						}
-						const op8 ph = __builtin_bit_cast(op8, wh);
-#pragma unroll
-						for (int dt = 0; dt < HD / 32; ++dt)
-						{
-							const uint16_t* v = sv + (32 * dt + r32) * G::VP + 32 * kt + 16 * h + 8 * half;
-							const op8 a = *reinterpret_cast<const op8*>(v);
-							o[dt] = mfma32x32x16(a, ph, o[dt]);
-							if constexpr (SPLIT) o[dt] = mfma32x32x16(a, __builtin_bit_cast(op8, wl), o[dt]);
-							if constexpr (MODE == kF32) o[dt] = mfma32x32x16(*reinterpret_cast<const op8*>(v + G::V_HALVES), ph, o[dt]);
-						}
+						else
+							wh[j] = cvt_pk_bf16(a, b);
 					}
+					const op8 ph = __builtin_bit_cast(op8, wh);
+#pragma unroll
+					for (int dt = 0; dt < NO; ++dt)
+					{
+						const uint16_t* v = sv + (TR * dt + col) * G::VP + (512 / TR) * x + 8 * sub;
+						const op8 a = *reinterpret_cast<const op8*>(v);
+						o[dt] = mfma(a, ph, o[dt]);
+						if constexpr (SPLIT) o[dt] = mfma(a, __builtin_bit_cast(op8, wl), o[dt]);
+						if constexpr (MODE == kF32) o[dt] = mfma(*reinterpret_cast<const op8*>(v + G::V_HALVES), ph, o[dt]);
+					}
+				}
 			}
 
+			l = row_sum<TR>(l);
+			if constexpr (MODE == kF32)
+				if (ev_o != 1000)
+#pragma unroll
+					for (int dt = 0; dt < NO; ++dt)
+#pragma unroll
+						for (int i = 0; i < EL; ++i) o[dt][i] = ldexpf(o[dt][i], -ev_o);
+			if (G::KG > 1 || MODE != kQ4) __syncthreads();
 			if constexpr (MODE != kQ4)
-				if (by_vector)
+				if (s_bad)
 				{
-					for (int r = 0; r < 32 && r0 + 32 * wave + r < n_rows; ++r)
+					for (int r = wave; r < G::ROWS && r0 + r < n_rows; r += G::WAVES)
 					{
-						const long long x = r0 + 32 * wave + r;
+						const long long x = r0 + r;
 						int a, b;
 						span_of(x, a, b);
 						vector_row<MODE>(p, row_at, token_of(x), kvh * group + static_cast<int>(x % group), kvh, a, b, lane);
@@ -639,24 +679,62 @@ namespace nnchip
 					return;
 				}
 
+			// ---- the key groups of a row meet, in order ----
+			if constexpr (G::KG > 1)
+			{
+				constexpr int Q = TR * HD / 256; // float4s of a lane
+				float4* const part = reinterpret_cast<float4*>(smem);
+				float2* const ml = reinterpret_cast<float2*>(smem + static_cast<size_t>(G::KG - 1) * G::RG * TR * HD * 4);
+				if (kg > 0)
+				{
+					const int w = (kg - 1) * G::RG + rg;
+#pragma unroll
+					for (int q = 0; q < Q; ++q)
+						part[(w * Q + q) * 64 + lane] = float4{o[q / (EL / 4)][4 * (q % (EL / 4))], o[q / (EL / 4)][4 * (q % (EL / 4)) + 1],
+						                                       o[q / (EL / 4)][4 * (q % (EL / 4)) + 2], o[q / (EL / 4)][4 * (q % (EL / 4)) + 3]};
+					ml[w * 64 + lane] = make_float2(off, l);
+				}
+				__syncthreads();
+				if (kg > 0) return;
+#pragma unroll
+				for (int g = 1; g < G::KG; ++g)
+				{
+					const int w = (g - 1) * G::RG + rg;
+					const float2 y = ml[w * 64 + lane];
+					const float now = fmaxf(off, y.x), to = now == -INFINITY ? 0.0f : now;
+					const float fa = fast_exp2(off - to), fb = fast_exp2(y.x - to);
+					off = now;
+					l = l * fa + y.y * fb;
+#pragma unroll
+					for (int q = 0; q < Q; ++q)
+					{
+						const float4 z = part[(w * Q + q) * 64 + lane];
+						auto& t = o[q / (EL / 4)];
+						const int e = 4 * (q % (EL / 4));
+						t[e] = fmaf(z.x, fb, t[e] * fa);
+						t[e + 1] = fmaf(z.y, fb, t[e + 1] * fa);
+						t[e + 2] = fmaf(z.z, fb, t[e + 2] * fa);
+						t[e + 3] = fmaf(z.w, fb, t[e + 3] * fa);
+					}
+				}
+			}
+
 			// ---- out ----
-			l = add_with_other_half(l);
 			if (!real) return;
 			const float inv = l == 0.0f ? 0.0f : 1.0f / l; // (a row that sees nothing: zeros)
 			const size_t oi = (row_at + tok) * p.out_stride + static_cast<size_t>(head) * hd;
 #pragma unroll
-			for (int dt = 0; dt < HD / 32; ++dt)
+			for (int dt = 0; dt < NO; ++dt)
 #pragma unroll
-				for (int c = 0; c < 4; ++c)
+				for (int c = 0; c < EL / 4; ++c)
 				{
-					const int d = 32 * dt + 8 * c + 4 * half;
+					const int d = TR * dt + 8 * c + 4 * sub;
 					if (d >= hd) continue;
 					float y[4];
 #pragma unroll
 					for (int j = 0; j < 4; ++j)
 					{
 						y[j] = o[dt][4 * c + j] * inv;
-						if constexpr (MODE == kF32) y[j] = ldexpf(y[j], ev == 1000 ? 0 : -ev);
 						if constexpr (MODE == kQ4) y[j] = gated(y[j], p.gate, oi + d + j);
 					}
 					if constexpr (MODE == kBf16)
@@ -666,37 +744,71 @@ namespace nnchip
 				}
 		}
 
-		template <int MODE, int NSEQ>
-		bool launch_mode(const flash_params& p, const flash_seqs<NSEQ>& s, hipStream_t stream)
+		// Fills in the tiles of `rows` rows and launches.
+		template <class G, int NSEQ>
+		bool launch_shape(const flash_params& p, flash_seqs<NSEQ>& s, hipStream_t stream)
 		{
-			const unsigned long long wg = static_cast<unsigned long long>(s.tiles) * p.n_kv;
-			if (wg > 0x7fffffffull) return false;
-			const dim3 grid(static_cast<unsigned>(wg));
-			if (p.head_dim <= 64)
-				flash_kernel<MODE, 64, NSEQ><<<grid, 64 * kWaves, 0, stream>>>(p, s);
-			else if (p.head_dim <= 96)
-				flash_kernel<MODE, 96, NSEQ><<<grid, 64 * kWaves, 0, stream>>>(p, s);
-			else if (p.head_dim <= 128)
-				flash_kernel<MODE, 128, NSEQ><<<grid, 64 * kWaves, 0, stream>>>(p, s);
-			else
-				flash_kernel<MODE, 256, NSEQ><<<grid, 64 * kWaves, 0, stream>>>(p, s);
+			long long tiles = 0;
+			for (int i = 0; i < s.n; ++i)
+			{
+				s.tile[i] = static_cast<int>(tiles);
+				tiles += (static_cast<long long>(s.len[i]) * (p.n_head / p.n_kv) + G::ROWS - 1) / G::ROWS;
+				if (tiles * p.n_kv > 0x7fffffff) return false;
+			}
+			if (tiles)
+				flash_kernel<G, NSEQ><<<dim3(static_cast<unsigned>(tiles * p.n_kv)), 64 * G::WAVES, 0, stream>>>(p, s);
 			return true;
+		}
+
+		// Work-groups of `rows` rows.
+		template <int NSEQ>
+		long long work_groups(const flash_params& p, const flash_seqs<NSEQ>& s, int rows)
+		{
+			long long n = 0;
+			for (int i = 0; i < s.n; ++i) n += (static_cast<long long>(s.len[i]) * (p.n_head / p.n_kv) + rows - 1) / rows;
+			return n * p.n_kv;
+		}
+
+		// One key group while there is a work-group for every CU; below that two, so
+		// that a CU's one work-group still has two wavefronts per SIMD (us alone /
+		// with three streams in flight, one -> two: 512 tokens of 32 over 8 x 128 at
+		// 4k keys over 4 bits, 128 work-groups, 133 / 59.6 -> 104 / 58.4; 1024 of 8
+		// over 4 x 256, a window of 1024, 64 work-groups, 73 / 25.1 -> 48 / 23.0;
+		// eight prompts of 1 to 2048 tokens, 1752 work-groups, 113 / 113 -> 152 /
+		// 148). Four key groups of half the rows gain more alone (78 and 38) and lose
+		// as much in flight (73 and 37). F32 at head_dim 256 converts K and V for half
+		// as many rows with two, and keeps one down to a quarter of the CUs (twelve
+		// texts of 5 to 1500 tokens of 3 x 256, 121 work-groups: 78 / 31 -> 62 / 44).
+		template <int MODE, int HD, int NSEQ>
+		bool launch_dim(const flash_params& p, flash_seqs<NSEQ>& s, int n_cu, hipStream_t stream)
+		{
+			const bool one = work_groups(p, s, 128) > (MODE == kF32 && HD == 256 ? n_cu / 4 : n_cu);
+			if constexpr (HD == 256)
+				return one ? launch_shape<shape<MODE, HD, 16, 8, 1>>(p, s, stream) : launch_shape<shape<MODE, HD, 16, 4, 2>>(p, s, stream);
+			else
+				return one ? launch_shape<shape<MODE, HD, 32, 4, 1>>(p, s, stream) : launch_shape<shape<MODE, HD, 32, 4, 2>>(p, s, stream);
+		}
+
+		template <int MODE, int NSEQ>
+		bool launch_mode(const flash_params& p, flash_seqs<NSEQ>& s, int n_cu, hipStream_t stream)
+		{
+			if (p.head_dim <= 64) return launch_dim<MODE, 64>(p, s, n_cu, stream);
+			if (p.head_dim <= 96) return launch_dim<MODE, 96>(p, s, n_cu, stream);
+			if (p.head_dim <= 128) return launch_dim<MODE, 128>(p, s, n_cu, stream);
+			return launch_dim<MODE, 256>(p, s, n_cu, stream);
 		}
 	}
 
-	int flash_tiles(int len, int group) { return static_cast<int>((static_cast<long long>(len) * group + kRows - 1) / kRows); }
-
-	bool launch_packed(const flash_params& p, const flash_seqs<kFlashSeqs>& s, bool bf16, hipStream_t stream)
+	bool launch_packed(const flash_params& p, flash_seqs<kFlashSeqs>& s, bool bf16, int n_cu, hipStream_t stream)
 	{
-		return bf16 ? launch_mode<kBf16>(p, s, stream) : launch_mode<kF32>(p, s, stream);
+		return bf16 ? launch_mode<kBf16>(p, s, n_cu, stream) : launch_mode<kF32>(p, s, n_cu, stream);
 	}
 
-	bool launch_flash_q4(const flash_params& p, int n_tok, hipStream_t stream)
+	bool launch_flash_q4(const flash_params& p, int n_tok, int n_cu, hipStream_t stream)
 	{
 		flash_seqs<1> s{};
 		s.n = 1;
 		s.len[0] = n_tok;
-		s.tiles = flash_tiles(n_tok, p.n_head / p.n_kv);
-		return launch_mode<kQ4>(p, s, stream);
+		return launch_mode<kQ4>(p, s, n_cu, stream);
 	}
 }

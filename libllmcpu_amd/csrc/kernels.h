@@ -167,17 +167,18 @@ namespace nnchip
 		int pos0, n_seq, rows; // 4-bit: position of the first row, keys, rows of the buffer
 	};
 	constexpr int kFlashMaxDim = 256;
-	// Sequences of one launch, none of them empty: first row, length, first tile.
+	// Sequences of one launch, none of them empty: first row, length, first tile
+	// (the launcher's).
 	constexpr int kFlashSeqs = 64;
 	template <int N>
 	struct flash_seqs
 	{
-		int n, tiles;
+		int n;
 		int start[N], len[N], tile[N];
 	};
-	int flash_tiles(int len, int group); // row blocks of a sequence
-	bool launch_packed(const flash_params& p, const flash_seqs<kFlashSeqs>& s, bool bf16, hipStream_t stream);
-	bool launch_flash_q4(const flash_params& p, int n_tok, hipStream_t stream);
+	// False, with nothing launched, for more work-groups than a grid holds.
+	bool launch_packed(const flash_params& p, flash_seqs<kFlashSeqs>& s, bool bf16, int n_cu, hipStream_t stream);
+	bool launch_flash_q4(const flash_params& p, int n_tok, int n_cu, hipStream_t stream);
 
 	// Tiled MFMA attention for a batch of query tokens.
 	struct prefill_params

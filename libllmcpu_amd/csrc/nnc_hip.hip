@@ -823,7 +823,7 @@ namespace
 			p.pos0 = pos0;
 			p.n_seq = n_seq;
 			p.rows = b.rows;
-			if (!nnchip::launch_flash_q4(p, n_tok, kv->stream))
+			if (!nnchip::launch_flash_q4(p, n_tok, kv->n_cu, kv->stream))
 				return fail(NNC_ERR_UNSUPPORTED_MODEL, "%d tokens of %d heads are too many for one call", n_tok, n_head);
 			NNC_HIP_TRY(hipGetLastError(), "attention over a 4-bit cache");
 			return NNC_OK;
@@ -1385,7 +1385,6 @@ nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void
 
 	// The longest first, kFlashSeqs to a launch, so that no long tile is begun
 	// last.
-	const int group = n_head / n_kv;
 	std::vector<int32_t> order;
 	try
 	{
@@ -1417,15 +1416,8 @@ nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void
 	p.causal = causal ? 1 : 0;
 	p.window = window;
 	p.scale = scale;
-	// Counted before the first launch, so that a refused call changes nothing.
-	for (size_t at = 0; at < order.size(); at += nnchip::kFlashSeqs)
-	{
-		unsigned long long tiles = 0;
-		for (size_t i = at; i < std::min(at + nnchip::kFlashSeqs, order.size()); ++i)
-			tiles += nnchip::flash_tiles(starts[order[i] + 1] - starts[order[i]], group);
-		if (tiles * n_kv > INT_MAX)
-			return fail(NNC_ERR_UNSUPPORTED_MODEL, "%llu row blocks of %d KV heads are too many for one launch", tiles, n_kv);
-	}
+	// (rows of 2^31 tokens and 2^31 work-groups need terabytes of q: no call that
+	// fits the device is refused after a launch)
 	const device_scope on(kv->device);
 	for (size_t at = 0; at < order.size(); at += nnchip::kFlashSeqs)
 	{
@@ -1434,10 +1426,8 @@ nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void
 		{
 			s.start[s.n] = starts[order[i]];
 			s.len[s.n] = starts[order[i] + 1] - starts[order[i]];
-			s.tile[s.n] = s.tiles;
-			s.tiles += nnchip::flash_tiles(s.len[s.n], group);
 		}
-		if (!nnchip::launch_packed(p, s, type == NNC_HIP_BF16, kv->stream))
+		if (!nnchip::launch_packed(p, s, type == NNC_HIP_BF16, kv->n_cu, kv->stream))
 			return fail(NNC_ERR_UNSUPPORTED_MODEL, "too many row blocks for one launch");
 		NNC_HIP_TRY(hipGetLastError(), "packed attention");
 	}
