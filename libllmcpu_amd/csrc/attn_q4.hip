@@ -18,8 +18,6 @@
 #include "kernels.h"
 #include "kv_q4.h"
 
-#include <type_traits>
-
 namespace nnchip
 {
 	namespace
@@ -78,8 +76,17 @@ namespace nnchip
 			return as_u32(is_lo ? l : h);
 		}
 
-		// Two wavefronts per SIMD where their registers fit (256 each).
-		constexpr int q4_per_simd(int nb, int t) { return nb <= 4 && nb * t <= 6 ? 2 : 1; }
+		// From the largest magnitude of a pair's q: the power of two (with the scale's
+		// sign: a masked score must stay the least) that brings it under 2^15, and
+		// what its scores are multiplied with afterwards. 0, infinity and NaN stay as
+		// they are.
+		__device__ __forceinline__ void q_scale(float qscale, float m, float& back, float& up)
+		{
+			int e = m > 0.0f && m < INFINITY ? 14 - ilogbf(m) : 0;
+			e = e < 126 ? e : 126;
+			back = fmaxf(ldexpf(fabsf(qscale), -e), 1.17549435e-38f);
+			up = ldexpf(qscale < 0.0f ? -1.0f : 1.0f, e);
+		}
 
 		__device__ __forceinline__ void add_scaled(float4& acc, const float4& v, float w)
 		{
@@ -97,6 +104,50 @@ namespace nnchip
 			if (p.gate) y = float4{gated(y.x, p.gate, at), gated(y.y, p.gate, at + 1), gated(y.z, p.gate, at + 2), gated(y.w, p.gate, at + 3)};
 			*reinterpret_cast<float4*>(p.out + at) = y;
 		}
+
+		// What the wavefronts (classes) of a work-group add up to, in their order.
+		struct joined
+		{
+			float m = -INFINITY, l = 0.0f;
+			float4 o = {0, 0, 0, 0};
+			__device__ __forceinline__ void factors(float mv, float& fa, float& fb)
+			{
+				const float now = fmaxf(m, mv), at = now == -INFINITY ? 0.0f : now;
+				fa = fast_exp2(m - at);
+				fb = fast_exp2(mv - at);
+				m = now;
+			}
+			__device__ __forceinline__ void add(float mv, float lv, const float4& v)
+			{
+				float fa, fb;
+				factors(mv, fa, fb);
+				l = fmaf(lv, fb, l * fa);
+				o = join4(o, fa, v, fb);
+			}
+			static __device__ __forceinline__ float4 join4(const float4& a, float fa, const float4& b, float fb)
+			{
+				return float4{fmaf(b.x, fb, a.x * fa), fmaf(b.y, fb, a.y * fa), fmaf(b.z, fb, a.z * fa), fmaf(b.w, fb, a.w * fa)};
+			}
+		};
+
+		// Elements d .. d + 3 of a pair's result over the split: its partial, or with
+		// one split the output.
+		template <int HD>
+		__device__ __forceinline__ void write_pair(const decode_params& p, int tok, int kvh, int h, int group, int split, int d,
+		                                           const float4& o, float m, float l)
+		{
+			if (p.n_split > 1)
+			{
+				float* dst = p.part + (((static_cast<size_t>(tok) * p.n_kv + kvh) * p.n_split + split) * group + h) * (HD + 4);
+				*reinterpret_cast<float4*>(dst + d) = o;
+				if (d == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(m, l);
+			}
+			else
+				write_out(p, (static_cast<size_t>(tok) * p.n_head + kvh * group + h) * HD + d, o, l);
+		}
+
+		// Two wavefronts per SIMD where their registers fit (256 each).
+		constexpr int q4_per_simd(int nb, int t) { return nb <= 4 && nb * t <= 6 ? 2 : 1; }
 
 		template <int NB, int T>
 		__global__ __launch_bounds__(64 * kW, q4_per_simd(NB, T)) void decode_q4_kernel(
@@ -145,7 +196,7 @@ namespace nnchip
 
 			// Q: per pair brought under 2^15 by a power of two, then fp16 hi or lo.
 			f16x8 q[T][NB];
-			float back[T]; // 2^-that power, and log2(e) * |scale| (its sign is in q: a masked score stays the least)
+			float back[T];
 			int first[T], last[T];
 #pragma unroll
 			for (int i = 0; i < T; ++i)
@@ -169,11 +220,8 @@ namespace nnchip
 					for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[b][j]));
 				}
 				m = column_max(m);
-				// (0, infinity and NaN: as they are)
-				int e = m > 0.0f && m < INFINITY ? 14 - ilogbf(m) : 0;
-				e = e < 126 ? e : 126;
-				back[i] = fmaxf(ldexpf(fabsf(p.qscale), -e), 1.17549435e-38f);
-				const float up = ldexpf(p.qscale < 0.0f ? -1.0f : 1.0f, e);
+				float up;
+				q_scale(p.qscale, m, back[i], up);
 #pragma unroll
 				for (int b = 0; b < NB; ++b)
 				{
@@ -308,29 +356,271 @@ namespace nnchip
 				{
 					const int c = x / (HD / 4), d = 4 * (x % (HD / 4)), pair = pair0 + c;
 					const int tok = p.n_tok == 1 ? 0 : pair / group, h = pair - tok * group;
-					float mx = s_o[0][c][HD];
-#pragma unroll
-					for (int v = 1; v < kW; ++v) mx = fmaxf(mx, s_o[v][c][HD]);
-					const float off = mx == -INFINITY ? 0.0f : mx;
-					float4 acc = {0, 0, 0, 0};
-					float sum = 0.0f;
+					joined y;
 #pragma unroll
 					for (int v = 0; v < kW; ++v)
-					{
-						const float f = fast_exp2(s_o[v][c][HD] - off);
-						add_scaled(acc, *reinterpret_cast<const float4*>(&s_o[v][c][d]), f);
-						sum = fmaf(s_o[v][c][HD + 1], f, sum);
-					}
-					if (p.n_split > 1)
-					{
-						float* dst = p.part + (((static_cast<size_t>(tok) * p.n_kv + kvh) * p.n_split + split) * group + h) * (HD + 4);
-						*reinterpret_cast<float4*>(dst + d) = acc;
-						if (d == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(mx, sum);
-					}
-					else
-						write_out(p, (static_cast<size_t>(tok) * p.n_head + kvh * group + h) * HD + d, acc, sum);
+						y.add(s_o[v][c][HD], s_o[v][c][HD + 1], *reinterpret_cast<const float4*>(&s_o[v][c][d]));
+					write_pair<HD>(p, tok, kvh, h, group, split, d, y.o, y.m, y.l);
 				}
 			}
+		}
+
+		// Many pairs (session batches, exact mode): a wavefront takes 16 pairs, one per
+		// column, their hi and lo parts in products of their own, and the work-group's
+		// four wavefronts share every value: each turns a quarter of a group's words
+		// into operands in LDS while they compute on the group before. The classes
+		// that decode_q4_kernel's wavefronts are (groups by their number in the split
+		// modulo kW) follow one another, with sums of their own, and join in the same
+		// order, so a pair gets the same bits. (With the kernel above, two tiles of 8
+		// pairs per wavefront, every tile's weights computed twice and every value
+		// made four times: 13 tokens of 32 over 8 x 128 at 20k keys 68 us a call.)
+		template <int NB>
+		__global__ __launch_bounds__(64 * kW, NB <= 4 ? 2 : 1) void decode_q4_multi_kernel(const decode_params p, int group)
+		{
+			constexpr int HD = NB * kQ4Block, UNITS = 2 * NB, OWN = (UNITS + kW - 1) / kW;
+			// unit u: K (even) or V (odd) of block u / 2, two operands of 1 KB
+			__shared__ __align__(16) unsigned char s_op[2][UNITS][2048];
+			const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+			const int split = blockIdx.x, kvh = blockIdx.y;
+			const int c = lane & 15, g = lane >> 4;
+			const int n_pairs = p.n_tok * group, pair0 = blockIdx.z * (16 * kW), mine0 = pair0 + 16 * wave;
+			const bool any = mine0 < n_pairs, real = mine0 + c < n_pairs;
+			const int pair = real ? mine0 + c : n_pairs - 1;
+			const int tok = pair / group, h = pair - tok * group;
+			int first, last, full_from, full_to, kmin, kmax, unused;
+			attn_span(p.causal, p.window, p.pos0 + tok, p.n_seq, first, last);
+			auto clamped = [&](int x) { return (x < n_pairs ? x : n_pairs - 1) / group; };
+			attn_span(p.causal, p.window, p.pos0 + clamped(mine0 + 15), p.n_seq, full_from, unused);
+			attn_span(p.causal, p.window, p.pos0 + clamped(mine0), p.n_seq, unused, full_to);
+			attn_span(p.causal, p.window, p.pos0 + clamped(pair0), p.n_seq, kmin, unused);
+			attn_span(p.causal, p.window, p.pos0 + clamped(pair0 + 16 * kW - 1), p.n_seq, unused, kmax);
+
+			const int k0 = p.split_base + split * p.split_keys;
+			const int g_base = k0 / kQ4Rows;
+			const int g_first = (kmin > k0 ? kmin : k0) / kQ4Rows;
+			const int g_last = (kmax < k0 + p.split_keys - 1 ? kmax : k0 + p.split_keys - 1) / kQ4Rows;
+			const int row_groups = p.rows / kQ4Rows, blocks = p.kv_dim / kQ4Block;
+			const unsigned char* recs = static_cast<const unsigned char*>(p.K) + static_cast<size_t>(kvh) * NB * kQ4Record;
+			const size_t group_bytes = static_cast<size_t>(blocks) * kQ4Record;
+			// The groups class by class.
+			auto class_first = [&](int cls)
+			{
+				const int at = g_base + cls;
+				return at >= g_first ? at : at + (g_first - at + kW - 1) / kW * kW;
+			};
+			struct place
+			{
+				int cls, kg;
+			};
+			auto next_of = [&](place x)
+			{
+				x.kg += kW;
+				while (x.kg > g_last && x.cls < kW - 1) x.kg = class_first(++x.cls);
+				if (x.kg > g_last) x.cls = kW;
+				return x;
+			};
+			place at{0, class_first(0) - kW};
+			at = next_of(at); // (cls kW: none)
+
+			// The wavefront's units of a group.
+			struct unit_regs
+			{
+				u32x2 code[OWN];
+				u32x4 s[OWN], z[OWN]; // (K: s.xy are the rows' (s, z))
+			};
+			auto load = [&](const place& x, unit_regs& r)
+			{
+				const unsigned char* rec0 = recs + static_cast<size_t>(x.kg % row_groups) * group_bytes;
+#pragma unroll
+				for (int n = 0; n < OWN; ++n)
+				{
+					const int u = wave + kW * n;
+					if (u >= UNITS) continue;
+					const unsigned char* rec = rec0 + (u >> 1) * kQ4Record;
+					if (u & 1)
+					{
+						r.code[n] = *reinterpret_cast<const u32x2*>(rec + 16 * lane + 8);
+						r.s[n] = *reinterpret_cast<const u32x4*>(rec + kQ4VScales + 32 * g);
+						r.z[n] = *reinterpret_cast<const u32x4*>(rec + kQ4VScales + 32 * g + 16);
+					}
+					else
+					{
+						r.code[n] = *reinterpret_cast<const u32x2*>(rec + 16 * lane);
+						const u32x2 sz = *reinterpret_cast<const u32x2*>(rec + kQ4KScales + 8 * c);
+						r.s[n] = u32x4{sz.x, sz.y, 0, 0};
+					}
+				}
+			};
+			const q4_masks masks;
+			auto convert = [&](const unit_regs& r, int buf)
+			{
+#pragma unroll
+				for (int n = 0; n < OWN; ++n)
+				{
+					const int u = wave + kW * n;
+					if (u >= UNITS) continue;
+#pragma unroll
+					for (int t = 0; t < 2; ++t)
+					{
+						const uint32_t w = t ? r.code[n].y : r.code[n].x;
+						const f16x8 x = u & 1 ? q4_v(w, r.s[n], r.z[n], masks) : q4_k(w, t ? r.s[n].y : r.s[n].x, masks);
+						*reinterpret_cast<f16x8*>(&s_op[buf][u][1024 * t + 16 * lane]) = x;
+					}
+				}
+			};
+			unit_regs regs;
+			const bool work = at.cls < kW;
+			if (work) load(at, regs);
+
+			// Q, as in decode_q4_kernel.
+			f16x8 qh[NB], ql[NB];
+			float back;
+			{
+				const float* src = p.q + (static_cast<size_t>(tok) * p.n_head + kvh * group + h) * HD + 8 * g;
+				float x[NB][8], m = 0.0f;
+#pragma unroll
+				for (int b = 0; b < NB; ++b)
+				{
+					const float4 u = *reinterpret_cast<const float4*>(src + 32 * b), v = *reinterpret_cast<const float4*>(src + 32 * b + 4);
+					x[b][0] = u.x, x[b][1] = v.x, x[b][2] = u.y, x[b][3] = v.y;
+					x[b][4] = u.z, x[b][5] = v.z, x[b][6] = u.w, x[b][7] = v.w;
+#pragma unroll
+					for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(x[b][j]));
+				}
+				float up;
+				q_scale(p.qscale, column_max(m), back, up);
+#pragma unroll
+				for (int b = 0; b < NB; ++b)
+				{
+					u32x4 hi, lo;
+#pragma unroll
+					for (int j = 0; j < 4; ++j)
+					{
+						hi[j] = part_of(x[b][2 * j] * up, x[b][2 * j + 1] * up, false);
+						lo[j] = part_of(x[b][2 * j] * up, x[b][2 * j + 1] * up, true);
+					}
+					qh[b] = as_f16x8(hi);
+					ql[b] = as_f16x8(lo);
+				}
+			}
+
+			f32x4 acc[NB][2] = {}, oh[NB][2] = {}, ol[NB][2] = {};
+			float m_all = -INFINITY, l_all = 0.0f, m_off = -INFINITY, l = 0.0f;
+			place ahead = at;
+			if (work)
+			{
+				convert(regs, 0);
+				ahead = next_of(at);
+				if (ahead.cls < kW) load(ahead, regs);
+			}
+			__syncthreads();
+			for (int buf = 0; at.cls < kW; buf ^= 1)
+			{
+				place then = ahead;
+				if (ahead.cls < kW)
+				{
+					convert(regs, buf ^ 1);
+					then = next_of(ahead);
+					if (then.cls < kW) load(then, regs);
+				}
+				if (any)
+				{
+					auto op = [&](int u, int t) { return *reinterpret_cast<const f16x8*>(&s_op[buf][u][1024 * t + 16 * lane]); };
+					f32x4 sh[2] = {}, sl[2] = {};
+#pragma unroll
+					for (int b = 0; b < NB; ++b)
+#pragma unroll
+						for (int t = 0; t < 2; ++t)
+						{
+							const f16x8 a = op(2 * b, t);
+							sh[t] = mfma16x16x32(a, qh[b], sh[t]);
+							sl[t] = mfma16x16x32(a, ql[b], sl[t]);
+						}
+					float sc[8];
+#pragma unroll
+					for (int j = 0; j < 8; ++j) sc[j] = sh[j >> 2][j & 3] + sl[j >> 2][j & 3];
+					const int key0 = at.kg * kQ4Rows;
+					if (key0 < full_from || key0 + kQ4Rows - 1 > full_to)
+					{
+						asm volatile("");
+#pragma unroll
+						for (int j = 0; j < 8; ++j)
+						{
+							const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+							if (key < first || key > last) sc[j] = -INFINITY;
+						}
+					}
+					float m = sc[0];
+#pragma unroll
+					for (int j = 1; j < 8; ++j) m = fmaxf(m, sc[j]);
+					m = column_max(m) * back;
+					const bool up = m > m_off + kRaise;
+					if (__any(up))
+					{
+						const float now = up ? m - kBelow : m_off;
+						const float f = up ? fast_exp2(m_off - now) : 1.0f;
+						m_off = now;
+						l *= f;
+#pragma unroll
+						for (int b = 0; b < NB; ++b) oh[b][0] *= f, oh[b][1] *= f, ol[b][0] *= f, ol[b][1] *= f;
+					}
+					const float off = m_off == -INFINITY ? 0.0f : m_off;
+#pragma unroll
+					for (int j = 0; j < 8; ++j)
+					{
+						sc[j] = fast_exp2(fmaf(sc[j], back, -off));
+						l += sc[j];
+					}
+					u32x4 hi, lo;
+#pragma unroll
+					for (int j = 0; j < 4; ++j)
+					{
+						hi[j] = part_of(sc[j], sc[4 + j], false);
+						lo[j] = part_of(sc[j], sc[4 + j], true);
+					}
+					const f16x8 wh = as_f16x8(hi), wl = as_f16x8(lo);
+#pragma unroll
+					for (int b = 0; b < NB; ++b)
+#pragma unroll
+						for (int t = 0; t < 2; ++t)
+						{
+							const f16x8 a = op(2 * b + 1, t);
+							oh[b][t] = mfma16x16x32(a, wh, oh[b][t]);
+							ol[b][t] = mfma16x16x32(a, wl, ol[b][t]);
+						}
+					if (ahead.cls != at.cls) // the class is done: it joins those before it
+					{
+						joined y;
+						y.m = m_all;
+						float fa, fb;
+						y.factors(m_off, fa, fb);
+						l_all = fmaf(column_sum(l), fb, l_all * fa);
+						m_all = y.m;
+						m_off = -INFINITY;
+						l = 0.0f;
+#pragma unroll
+						for (int b = 0; b < NB; ++b)
+#pragma unroll
+							for (int t = 0; t < 2; ++t)
+#pragma unroll
+								for (int j = 0; j < 4; ++j)
+								{
+									acc[b][t][j] = fmaf(oh[b][t][j] + ol[b][t][j], fb, acc[b][t][j] * fa);
+									oh[b][t][j] = ol[b][t][j] = 0.0f;
+								}
+					}
+				}
+				at = ahead;
+				ahead = then;
+				__syncthreads();
+			}
+			if (!real) return;
+#pragma unroll
+			for (int b = 0; b < NB; ++b)
+#pragma unroll
+				for (int t = 0; t < 2; ++t)
+					write_pair<HD>(p, tok, kvh, h, group, split, 32 * b + 16 * t + 4 * g,
+					               float4{acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]}, m_all, l_all);
 		}
 
 		// The ordered merge of a pair's splits: M = the largest offset, o and l summed
@@ -396,20 +686,19 @@ namespace nnchip
 		template <int NB>
 		void launch_nb(const decode_params& p, int n_tok, int group, hipStream_t stream)
 		{
-			// Several tiles share a work-group's records as far as the registers go.
-			constexpr int kMost = NB <= 3 ? 4 : NB <= 4 ? 2 : 1;
-			const int tiles = (n_tok * group + 7) / 8;
-			auto run = [&](auto t)
-			{
-				constexpr int T = decltype(t)::value;
-				decode_q4_kernel<NB, T><<<dim3(p.n_split, p.n_kv, (tiles + T - 1) / T), 64 * kW, 0, stream>>>(p, group);
-			};
-			if (tiles == 1 || kMost == 1)
-				run(std::integral_constant<int, 1>());
-			else if (tiles == 2 || kMost == 2)
-				run(std::integral_constant<int, kMost < 2 ? 1 : 2>());
-			else
-				run(std::integral_constant<int, kMost>());
+			// Up to 8 pairs a wavefront takes them all, up to 16 two tiles of 8 (or, where
+			// their registers do not fit, two work-groups); above that the kernel for
+			// many, whose registers do not fit at 16 blocks.
+			const int pairs = n_tok * group, tiles = (pairs + 7) / 8;
+			const dim3 threads(64 * kW);
+			if constexpr (NB <= 8)
+				if (pairs > 16)
+					decode_q4_multi_kernel<NB><<<dim3(p.n_split, p.n_kv, (pairs + 16 * kW - 1) / (16 * kW)), threads, 0, stream>>>(p, group);
+			if constexpr (NB <= 4)
+				if (pairs > 8 && pairs <= 16)
+					decode_q4_kernel<NB, 2><<<dim3(p.n_split, p.n_kv, 1), threads, 0, stream>>>(p, group);
+			if (pairs <= 8 || (NB > 4 && pairs <= 16) || NB > 8)
+				decode_q4_kernel<NB, 1><<<dim3(p.n_split, p.n_kv, tiles), threads, 0, stream>>>(p, group);
 			if (p.n_split > 1)
 				merge_q4_kernel<<<dim3(p.n_head, n_tok), kMergeThreads, 0, stream>>>(p, NB * kQ4Block, group);
 		}
