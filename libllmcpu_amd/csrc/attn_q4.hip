@@ -377,9 +377,9 @@ namespace nnchip
 		template <int NB>
 		__global__ __launch_bounds__(64 * kW, NB <= 4 ? 2 : 1) void decode_q4_multi_kernel(const decode_params p, int group)
 		{
-			constexpr int HD = NB * kQ4Block, UNITS = 2 * NB, OWN = (UNITS + kW - 1) / kW;
-			// unit u: K (even) or V (odd) of block u / 2, two operands of 1 KB
-			__shared__ __align__(16) unsigned char s_op[2][UNITS][2048];
+			constexpr int HD = NB * kQ4Block, OWN = (NB + 1) / 2, PER = NB <= 6 ? 2 : 1; // groups at a time
+			// Two buffers of PER groups: K and V of each block, two operands of 1 KB.
+			__shared__ __align__(16) unsigned char s_op[2][PER][2][NB][2048];
 			const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 			const int split = blockIdx.x, kvh = blockIdx.y;
 			const int c = lane & 15, g = lane >> 4;
@@ -422,55 +422,80 @@ namespace nnchip
 			place at{0, class_first(0) - kW};
 			at = next_of(at); // (cls kW: none)
 
-			// The wavefront's units of a group.
+			// Wavefronts 0 and 2 make K's operands, 1 and 3 V's, of every other block.
+			const bool is_v = wave & 1;
+			const int block0 = wave >> 1;
 			struct unit_regs
 			{
-				u32x2 code[OWN];
-				u32x4 s[OWN], z[OWN]; // (K: s.xy are the rows' (s, z))
+				u32x2 code[OWN], ksz[OWN];
+				u32x4 s[OWN], z[OWN];
 			};
 			auto load = [&](const place& x, unit_regs& r)
 			{
-				const unsigned char* rec0 = recs + static_cast<size_t>(x.kg % row_groups) * group_bytes;
-#pragma unroll
-				for (int n = 0; n < OWN; ++n)
+				if (x.cls >= kW) return;
+				const unsigned char* rec = recs + static_cast<size_t>(x.kg % row_groups) * group_bytes + block0 * kQ4Record;
+				if (is_v)
 				{
-					const int u = wave + kW * n;
-					if (u >= UNITS) continue;
-					const unsigned char* rec = rec0 + (u >> 1) * kQ4Record;
-					if (u & 1)
-					{
-						r.code[n] = *reinterpret_cast<const u32x2*>(rec + 16 * lane + 8);
-						r.s[n] = *reinterpret_cast<const u32x4*>(rec + kQ4VScales + 32 * g);
-						r.z[n] = *reinterpret_cast<const u32x4*>(rec + kQ4VScales + 32 * g + 16);
-					}
-					else
-					{
-						r.code[n] = *reinterpret_cast<const u32x2*>(rec + 16 * lane);
-						const u32x2 sz = *reinterpret_cast<const u32x2*>(rec + kQ4KScales + 8 * c);
-						r.s[n] = u32x4{sz.x, sz.y, 0, 0};
-					}
+#pragma unroll
+					for (int n = 0; n < OWN; ++n)
+						if (block0 + 2 * n < NB)
+						{
+							r.code[n] = *reinterpret_cast<const u32x2*>(rec + 2 * n * kQ4Record + 16 * lane + 8);
+							r.s[n] = *reinterpret_cast<const u32x4*>(rec + 2 * n * kQ4Record + kQ4VScales + 32 * g);
+							r.z[n] = *reinterpret_cast<const u32x4*>(rec + 2 * n * kQ4Record + kQ4VScales + 32 * g + 16);
+						}
+				}
+				else
+				{
+#pragma unroll
+					for (int n = 0; n < OWN; ++n)
+						if (block0 + 2 * n < NB)
+						{
+							r.code[n] = *reinterpret_cast<const u32x2*>(rec + 2 * n * kQ4Record + 16 * lane);
+							r.ksz[n] = *reinterpret_cast<const u32x2*>(rec + 2 * n * kQ4Record + kQ4KScales + 8 * c);
+						}
 				}
 			};
 			const q4_masks masks;
-			auto convert = [&](const unit_regs& r, int buf)
+			auto convert = [&](const place& x, const unit_regs& r, int buf, int slot)
 			{
-#pragma unroll
-				for (int n = 0; n < OWN; ++n)
+				if (x.cls >= kW) return;
+				if (is_v)
 				{
-					const int u = wave + kW * n;
-					if (u >= UNITS) continue;
 #pragma unroll
-					for (int t = 0; t < 2; ++t)
-					{
-						const uint32_t w = t ? r.code[n].y : r.code[n].x;
-						const f16x8 x = u & 1 ? q4_v(w, r.s[n], r.z[n], masks) : q4_k(w, t ? r.s[n].y : r.s[n].x, masks);
-						*reinterpret_cast<f16x8*>(&s_op[buf][u][1024 * t + 16 * lane]) = x;
-					}
+					for (int n = 0; n < OWN; ++n)
+						if (block0 + 2 * n < NB)
+						{
+							f16x8* to = reinterpret_cast<f16x8*>(&s_op[buf][slot][1][block0 + 2 * n][16 * lane]);
+							to[0] = q4_v(r.code[n].x, r.s[n], r.z[n], masks);
+							to[64] = q4_v(r.code[n].y, r.s[n], r.z[n], masks);
+						}
+				}
+				else
+				{
+#pragma unroll
+					for (int n = 0; n < OWN; ++n)
+						if (block0 + 2 * n < NB)
+						{
+							f16x8* to = reinterpret_cast<f16x8*>(&s_op[buf][slot][0][block0 + 2 * n][16 * lane]);
+							to[0] = q4_k(r.code[n].x, r.ksz[n].x, masks);
+							to[64] = q4_k(r.code[n].y, r.ksz[n].y, masks);
+						}
 				}
 			};
-			unit_regs regs;
-			const bool work = at.cls < kW;
-			if (work) load(at, regs);
+			// The groups PER at a time: now (in LDS), ahead (in registers).
+			auto after = [&](const place& x) { return x.cls < kW ? next_of(x) : x; };
+			place now[PER], ahead[PER];
+			auto follow = [&](place x, place* to)
+			{
+#pragma unroll
+				for (int i = 0; i < PER; ++i) to[i] = x = after(x);
+			};
+			unit_regs regs[PER];
+			now[0] = at;
+			if constexpr (PER == 2) now[1] = after(at);
+#pragma unroll
+			for (int i = 0; i < PER; ++i) load(now[i], regs[i]);
 
 			// Q, as in decode_q4_kernel.
 			f16x8 qh[NB], ql[NB];
@@ -506,112 +531,119 @@ namespace nnchip
 
 			f32x4 acc[NB][2] = {}, oh[NB][2] = {}, ol[NB][2] = {};
 			float m_all = -INFINITY, l_all = 0.0f, m_off = -INFINITY, l = 0.0f;
-			place ahead = at;
-			if (work)
-			{
-				convert(regs, 0);
-				ahead = next_of(at);
-				if (ahead.cls < kW) load(ahead, regs);
-			}
+			follow(now[PER - 1], ahead);
+#pragma unroll
+			for (int i = 0; i < PER; ++i) convert(now[i], regs[i], 0, i);
+#pragma unroll
+			for (int i = 0; i < PER; ++i) load(ahead[i], regs[i]);
 			__syncthreads();
-			for (int buf = 0; at.cls < kW; buf ^= 1)
+			for (int buf = 0; now[0].cls < kW; buf ^= 1)
 			{
-				place then = ahead;
-				if (ahead.cls < kW)
-				{
-					convert(regs, buf ^ 1);
-					then = next_of(ahead);
-					if (then.cls < kW) load(then, regs);
-				}
+#pragma unroll
+				for (int i = 0; i < PER; ++i) convert(ahead[i], regs[i], buf ^ 1, i);
+				place then[PER];
+				follow(ahead[PER - 1], then);
+#pragma unroll
+				for (int i = 0; i < PER; ++i) load(then[i], regs[i]);
 				if (any)
 				{
-					auto op = [&](int u, int t) { return *reinterpret_cast<const f16x8*>(&s_op[buf][u][1024 * t + 16 * lane]); };
-					f32x4 sh[2] = {}, sl[2] = {};
+					auto op = [&](int slot, int v, int b, int t) { return *reinterpret_cast<const f16x8*>(&s_op[buf][slot][v][b][1024 * t + 16 * lane]); };
+					float sc[PER][8];
 #pragma unroll
-					for (int b = 0; b < NB; ++b)
-#pragma unroll
-						for (int t = 0; t < 2; ++t)
-						{
-							const f16x8 a = op(2 * b, t);
-							sh[t] = mfma16x16x32(a, qh[b], sh[t]);
-							sl[t] = mfma16x16x32(a, ql[b], sl[t]);
-						}
-					float sc[8];
-#pragma unroll
-					for (int j = 0; j < 8; ++j) sc[j] = sh[j >> 2][j & 3] + sl[j >> 2][j & 3];
-					const int key0 = at.kg * kQ4Rows;
-					if (key0 < full_from || key0 + kQ4Rows - 1 > full_to)
+					for (int x = 0; x < PER; ++x)
 					{
-						asm volatile("");
-#pragma unroll
-						for (int j = 0; j < 8; ++j)
-						{
-							const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
-							if (key < first || key > last) sc[j] = -INFINITY;
-						}
-					}
-					float m = sc[0];
-#pragma unroll
-					for (int j = 1; j < 8; ++j) m = fmaxf(m, sc[j]);
-					m = column_max(m) * back;
-					const bool up = m > m_off + kRaise;
-					if (__any(up))
-					{
-						const float now = up ? m - kBelow : m_off;
-						const float f = up ? fast_exp2(m_off - now) : 1.0f;
-						m_off = now;
-						l *= f;
-#pragma unroll
-						for (int b = 0; b < NB; ++b) oh[b][0] *= f, oh[b][1] *= f, ol[b][0] *= f, ol[b][1] *= f;
-					}
-					const float off = m_off == -INFINITY ? 0.0f : m_off;
-#pragma unroll
-					for (int j = 0; j < 8; ++j)
-					{
-						sc[j] = fast_exp2(fmaf(sc[j], back, -off));
-						l += sc[j];
-					}
-					u32x4 hi, lo;
-#pragma unroll
-					for (int j = 0; j < 4; ++j)
-					{
-						hi[j] = part_of(sc[j], sc[4 + j], false);
-						lo[j] = part_of(sc[j], sc[4 + j], true);
-					}
-					const f16x8 wh = as_f16x8(hi), wl = as_f16x8(lo);
-#pragma unroll
-					for (int b = 0; b < NB; ++b)
-#pragma unroll
-						for (int t = 0; t < 2; ++t)
-						{
-							const f16x8 a = op(2 * b + 1, t);
-							oh[b][t] = mfma16x16x32(a, wh, oh[b][t]);
-							ol[b][t] = mfma16x16x32(a, wl, ol[b][t]);
-						}
-					if (ahead.cls != at.cls) // the class is done: it joins those before it
-					{
-						joined y;
-						y.m = m_all;
-						float fa, fb;
-						y.factors(m_off, fa, fb);
-						l_all = fmaf(column_sum(l), fb, l_all * fa);
-						m_all = y.m;
-						m_off = -INFINITY;
-						l = 0.0f;
+						if (now[x].cls >= kW) continue;
+						f32x4 sh[2] = {}, sl[2] = {};
 #pragma unroll
 						for (int b = 0; b < NB; ++b)
 #pragma unroll
 							for (int t = 0; t < 2; ++t)
+							{
+								const f16x8 a = op(x, 0, b, t);
+								sh[t] = mfma16x16x32(a, qh[b], sh[t]);
+								sl[t] = mfma16x16x32(a, ql[b], sl[t]);
+							}
 #pragma unroll
-								for (int j = 0; j < 4; ++j)
-								{
-									acc[b][t][j] = fmaf(oh[b][t][j] + ol[b][t][j], fb, acc[b][t][j] * fa);
-									oh[b][t][j] = ol[b][t][j] = 0.0f;
-								}
+						for (int j = 0; j < 8; ++j) sc[x][j] = sh[j >> 2][j & 3] + sl[j >> 2][j & 3];
+					}
+#pragma unroll
+					for (int x = 0; x < PER; ++x)
+					{
+						if (now[x].cls >= kW) continue;
+						const int key0 = now[x].kg * kQ4Rows;
+						if (key0 < full_from || key0 + kQ4Rows - 1 > full_to)
+						{
+							asm volatile("");
+#pragma unroll
+							for (int j = 0; j < 8; ++j)
+							{
+								const int key = key0 + 16 * (j >> 2) + 4 * g + (j & 3);
+								if (key < first || key > last) sc[x][j] = -INFINITY;
+							}
+						}
+						float m = sc[x][0];
+#pragma unroll
+						for (int j = 1; j < 8; ++j) m = fmaxf(m, sc[x][j]);
+						m = column_max(m) * back;
+						const bool up = m > m_off + kRaise;
+						if (__any(up))
+						{
+							const float to = up ? m - kBelow : m_off;
+							const float f = up ? fast_exp2(m_off - to) : 1.0f;
+							m_off = to;
+							l *= f;
+#pragma unroll
+							for (int b = 0; b < NB; ++b) oh[b][0] *= f, oh[b][1] *= f, ol[b][0] *= f, ol[b][1] *= f;
+						}
+						const float off = m_off == -INFINITY ? 0.0f : m_off;
+#pragma unroll
+						for (int j = 0; j < 8; ++j)
+						{
+							sc[x][j] = fast_exp2(fmaf(sc[x][j], back, -off));
+							l += sc[x][j];
+						}
+						u32x4 hi, lo;
+#pragma unroll
+						for (int j = 0; j < 4; ++j)
+						{
+							hi[j] = part_of(sc[x][j], sc[x][4 + j], false);
+							lo[j] = part_of(sc[x][j], sc[x][4 + j], true);
+						}
+						const f16x8 wh = as_f16x8(hi), wl = as_f16x8(lo);
+#pragma unroll
+						for (int b = 0; b < NB; ++b)
+#pragma unroll
+							for (int t = 0; t < 2; ++t)
+							{
+								const f16x8 a = op(x, 1, b, t);
+								oh[b][t] = mfma16x16x32(a, wh, oh[b][t]);
+								ol[b][t] = mfma16x16x32(a, wl, ol[b][t]);
+							}
+						if ((x + 1 < PER ? now[(x + 1) % PER].cls : ahead[0].cls) != now[x].cls) // the class is done: it joins those before it
+						{
+							joined y;
+							y.m = m_all;
+							float fa, fb;
+							y.factors(m_off, fa, fb);
+							l_all = fmaf(column_sum(l), fb, l_all * fa);
+							m_all = y.m;
+							m_off = -INFINITY;
+							l = 0.0f;
+#pragma unroll
+							for (int b = 0; b < NB; ++b)
+#pragma unroll
+								for (int t = 0; t < 2; ++t)
+#pragma unroll
+									for (int j = 0; j < 4; ++j)
+									{
+										acc[b][t][j] = fmaf(oh[b][t][j] + ol[b][t][j], fb, acc[b][t][j] * fa);
+										oh[b][t][j] = ol[b][t][j] = 0.0f;
+									}
+						}
 					}
 				}
-				at = ahead;
-				ahead = then;
+#pragma unroll
+				for (int i = 0; i < PER; ++i) now[i] = ahead[i], ahead[i] = then[i];
 				__syncthreads();
 			}
 			if (!real) return;
