@@ -146,10 +146,163 @@ namespace nnchip
 				write_out(p, (static_cast<size_t>(tok) * p.n_head + kvh * group + h) * HD + d, o, l);
 		}
 
+		// The ordered merge of a pair's splits: M = the largest offset; o and l
+		// relative to it, summed over the splits of a slice in ascending order, then
+		// over the slices in order. Split s (its absolute number: keys / split_keys)
+		// belongs to slice s % merge_slices, so a batch whose first split lies before a
+		// token's own gives the token the same sums (those splits add exact zeros).
+		constexpr int kMergeThreads = 256, kMergeAhead = 8;
+		static_assert(kDecodeMaxSplits == kMergeThreads, "a thread per split");
+		__host__ __device__ constexpr int merge_slices(int hd) { return kMergeThreads / (hd / 4); }
+
+		// By 256 threads per pair: every split's offset in one load per thread, outputs
+		// in float4 columns times slices.
+		__global__ __launch_bounds__(kMergeThreads) void merge_q4_kernel(const decode_params p, int hd, int group)
+		{
+			__shared__ float s_f[kDecodeMaxSplits], s_lf[kDecodeMaxSplits];
+			__shared__ float s_red[kMergeThreads / 64];
+			__shared__ float s_l[kMergeThreads];
+			__shared__ float4 s_o[kMergeThreads];
+			const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+			const int qh = blockIdx.x, tok = blockIdx.y, kvh = qh / group, h = qh % group;
+			const int ns = p.n_split, cols = hd / 4, n_slices = merge_slices(hd);
+			const int c = tid % cols, slice = tid / cols;
+			const int base = p.split_base / p.split_keys; // the first split's number
+			const int s0 = n_slices - 1 - (base + n_slices - 1 - slice) % n_slices; // the slice's first split
+			const float* part = p.part + ((static_cast<size_t>(tok) * p.n_kv + kvh) * ns * group + h) * (hd + 4);
+			const size_t step = static_cast<size_t>(group) * (hd + 4);
+
+			float2 ml = make_float2(-INFINITY, 0.0f);
+			if (tid < ns) ml = *reinterpret_cast<const float2*>(part + tid * step + hd);
+			float4 o[kMergeAhead]; // the slice's first splits, on their way meanwhile
+#pragma unroll
+			for (int i = 0; i < kMergeAhead; ++i)
+			{
+				const int s = s0 + i * n_slices;
+				o[i] = float4{0, 0, 0, 0};
+				if (slice < n_slices && s < ns) o[i] = *reinterpret_cast<const float4*>(part + s * step + 4 * c);
+			}
+			float mx = max_with_other_half(max_other_row(row_max(ml.x)));
+			if (lane == 0) s_red[wave] = mx;
+			__syncthreads();
+			mx = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+			const float f = fast_exp2(ml.x - (mx == -INFINITY ? 0.0f : mx));
+			s_f[tid] = f;
+			s_lf[tid] = ml.y;
+			__syncthreads();
+			float4 acc = {0, 0, 0, 0};
+			float l = 0.0f;
+			if (slice < n_slices)
+			{
+#pragma unroll
+				for (int i = 0; i < kMergeAhead; ++i)
+				{
+					const int s = s0 + i * n_slices;
+					if (s >= ns) continue;
+					add_scaled(acc, o[i], s_f[s]);
+					l = fmaf(s_lf[s], s_f[s], l);
+				}
+				for (int s = s0 + kMergeAhead * n_slices; s < ns; s += n_slices)
+				{
+					add_scaled(acc, *reinterpret_cast<const float4*>(part + s * step + 4 * c), s_f[s]);
+					l = fmaf(s_lf[s], s_f[s], l);
+				}
+			}
+			s_o[tid] = acc;
+			s_l[tid] = l;
+			__syncthreads();
+			if (tid >= cols) return;
+			acc = float4{0, 0, 0, 0};
+			l = 0.0f;
+			for (int i = 0; i < n_slices; ++i)
+			{
+				add_scaled(acc, s_o[i * cols + tid], 1.0f);
+				l += s_l[i * cols + tid];
+			}
+			write_out(p, (static_cast<size_t>(tok) * p.n_head + qh) * hd + 4 * tid, acc, l);
+		}
+
+		// The same within the split launch, for one token's pairs and at most
+		// kFuseSplits splits: a work-group's partial is stored with device scope (sc1:
+		// through its XCD's L2, acknowledged once every XCD can see it), then the
+		// work-group counts itself in; the last of its KV head to do so resets the
+		// count and merges, a float4 column of a pair per thread, every split's loads
+		// at once and with device scope.
+		constexpr int kAuxDevice = 16, kFuseSplits = 8;
+		__device__ __forceinline__ __amdgpu_buffer_rsrc_t head_partials(const decode_params& p, int kvh, int group, int hd)
+		{
+			const size_t floats = static_cast<size_t>(p.n_split) * group * (hd + 4);
+			return __builtin_amdgcn_make_buffer_rsrc(p.part + kvh * floats, 0, static_cast<int>(floats * 4), 0x00020000);
+		}
+		__device__ __forceinline__ void store_device(__amdgpu_buffer_rsrc_t r, int at, const float4& v)
+		{
+			__builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, 4 * at, 0, kAuxDevice);
+		}
+		template <int HD>
+		__device__ __forceinline__ void merge_last(const decode_params& p, int kvh, int group)
+		{
+			constexpr int COLS = HD / 4, SLICES = merge_slices(HD), CLASSES = SLICES < kFuseSplits ? SLICES : kFuseSplits;
+			const auto rs = head_partials(p, kvh, group, HD);
+			const int base = p.split_base / p.split_keys, ns = p.n_split;
+			for (int x = threadIdx.x; x < group * COLS; x += 64 * kW)
+			{
+				const int h = x / COLS, c = x % COLS;
+				float4 o[kFuseSplits];
+				float2 ml[kFuseSplits];
+#pragma unroll
+				for (int s = 0; s < kFuseSplits; ++s) // (past the last split: past the descriptor, zeros)
+				{
+					const int at = 4 * (s * group + h) * (HD + 4);
+					o[s] = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(rs, at + 16 * c, 0, kAuxDevice));
+					ml[s] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, at + 4 * HD, 0, kAuxDevice));
+				}
+				float mx = -INFINITY;
+#pragma unroll
+				for (int s = 0; s < kFuseSplits; ++s)
+				{
+					if (s >= ns) ml[s].x = -INFINITY;
+					mx = fmaxf(mx, ml[s].x);
+				}
+				const float off = mx == -INFINITY ? 0.0f : mx;
+				// Class k: splits k, k + SLICES, ..., which are slice (base + k) % SLICES.
+				float4 part[CLASSES];
+				float l[CLASSES];
+#pragma unroll
+				for (int k = 0; k < CLASSES; ++k)
+				{
+					part[k] = float4{0, 0, 0, 0};
+					l[k] = 0.0f;
+#pragma unroll
+					for (int s = k; s < kFuseSplits; s += SLICES)
+					{
+						if (s >= ns) continue;
+						const float f = fast_exp2(ml[s].x - off);
+						add_scaled(part[k], o[s], f);
+						l[k] = fmaf(ml[s].y, f, l[k]);
+					}
+				}
+				// The slices in order: from the class of slice 0 on, then the classes
+				// before it.
+				const int c0 = (SLICES - base % SLICES) % SLICES;
+				float4 acc = {0, 0, 0, 0};
+				float sum = 0.0f;
+#pragma unroll
+				for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+					for (int k = 0; k < CLASSES; ++k)
+						if ((k >= c0) == (pass == 0))
+						{
+							add_scaled(acc, part[k], 1.0f);
+							sum += l[k];
+						}
+				write_out(p, static_cast<size_t>(kvh * group + h) * HD + 4 * c, acc, sum);
+			}
+		}
+
 		// Two wavefronts per SIMD where their registers fit (256 each).
 		constexpr int q4_per_simd(int nb, int t) { return nb <= 4 && nb * t <= 6 ? 2 : 1; }
 
-		template <int NB, int T>
+		template <int NB, int T, bool FUSE>
 		__global__ __launch_bounds__(64 * kW, q4_per_simd(NB, T)) void decode_q4_kernel(
 			const decode_params p, int group)
 		{
@@ -360,8 +513,33 @@ namespace nnchip
 #pragma unroll
 					for (int v = 0; v < kW; ++v)
 						y.add(s_o[v][c][HD], s_o[v][c][HD + 1], *reinterpret_cast<const float4*>(&s_o[v][c][d]));
-					write_pair<HD>(p, tok, kvh, h, group, split, d, y.o, y.m, y.l);
+					if constexpr (FUSE)
+					{
+						const auto rs = head_partials(p, kvh, group, HD);
+						const int at = (split * group + h) * (HD + 4);
+						store_device(rs, at + d, y.o);
+						if (d == 0) store_device(rs, at + HD, float4{y.m, y.l, 0, 0});
+					}
+					else
+						write_pair<HD>(p, tok, kvh, h, group, split, d, y.o, y.m, y.l);
 				}
+			}
+			if constexpr (FUSE)
+			{
+				__shared__ int s_last;
+				asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the thread's stores are seen everywhere
+				__syncthreads();
+				if (threadIdx.x == 0)
+				{
+					unsigned* count = p.counts + kvh;
+					const bool is_last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+					                     static_cast<unsigned>(p.n_split - 1);
+					if (is_last) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+					s_last = is_last;
+				}
+				__syncthreads();
+				if (!s_last) return;
+				merge_last<HD>(p, kvh, group);
 			}
 		}
 
@@ -655,66 +833,6 @@ namespace nnchip
 					               float4{acc[b][t][0], acc[b][t][1], acc[b][t][2], acc[b][t][3]}, m_all, l_all);
 		}
 
-		// The ordered merge of a pair's splits: M = the largest offset, o and l summed
-		// relative to it. A work-group per (token, query head): every split's offset
-		// and sum in one load per thread, outputs in float4 columns times slices of
-		// the splits, joined in slice order. A split's thread and slice follow its
-		// absolute number (keys / split_keys), so a batch whose first split lies
-		// before a token's own gives the token the same sums (those splits add
-		// exact zeros).
-		constexpr int kMergeThreads = 256, kMergeAhead = 8;
-		static_assert(kDecodeMaxSplits == kMergeThreads, "a thread per split");
-		__global__ __launch_bounds__(kMergeThreads) void merge_q4_kernel(const decode_params p, int hd, int group)
-		{
-			__shared__ float s_f[kDecodeMaxSplits];
-			__shared__ float s_red[2][kMergeThreads / 64];
-			__shared__ float4 s_o[kMergeThreads];
-			const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-			const int qh = blockIdx.x, tok = blockIdx.y, kvh = qh / group, h = qh % group;
-			const int ns = p.n_split, cols = hd / 4, n_slices = kMergeThreads / cols;
-			const int c = tid % cols, slice = tid / cols;
-			const int base = p.split_base / p.split_keys; // the first split's number
-			const int mine = (tid - base) & (kDecodeMaxSplits - 1); // the thread's split
-			const int s0 = n_slices - 1 - (base + n_slices - 1 - slice) % n_slices; // the slice's first split
-			const float* part = p.part + ((static_cast<size_t>(tok) * p.n_kv + kvh) * ns * group + h) * (hd + 4);
-			const size_t step = static_cast<size_t>(group) * (hd + 4);
-
-			float m = -INFINITY, l = 0.0f;
-			if (mine < ns) m = part[mine * step + hd], l = part[mine * step + hd + 1];
-			float4 o[kMergeAhead]; // the slice's first splits, on their way meanwhile
-#pragma unroll
-			for (int i = 0; i < kMergeAhead; ++i)
-			{
-				const int s = s0 + i * n_slices;
-				o[i] = float4{0, 0, 0, 0};
-				if (slice < n_slices && s < ns) o[i] = *reinterpret_cast<const float4*>(part + s * step + 4 * c);
-			}
-			float mx = max_with_other_half(max_other_row(row_max(m)));
-			if (lane == 0) s_red[0][wave] = mx;
-			__syncthreads();
-			mx = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-			const float f = fast_exp2(m - (mx == -INFINITY ? 0.0f : mx));
-			s_f[mine] = f;
-			l = wave_sum_dpp(l * f);
-			if (lane == 0) s_red[1][wave] = l;
-			__syncthreads();
-			float4 acc = {0, 0, 0, 0};
-			if (slice < n_slices)
-			{
-#pragma unroll
-				for (int i = 0; i < kMergeAhead; ++i)
-					if (s0 + i * n_slices < ns) add_scaled(acc, o[i], s_f[s0 + i * n_slices]);
-				for (int s = s0 + kMergeAhead * n_slices; s < ns; s += n_slices)
-					add_scaled(acc, *reinterpret_cast<const float4*>(part + s * step + 4 * c), s_f[s]);
-			}
-			s_o[tid] = acc;
-			__syncthreads();
-			if (tid >= cols) return;
-			for (int i = 1; i < n_slices; ++i) add_scaled(acc, s_o[i * cols + tid], 1.0f);
-			const float sum = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
-			write_out(p, (static_cast<size_t>(tok) * p.n_head + qh) * hd + 4 * tid, acc, sum);
-		}
-
 		template <int NB>
 		void launch_nb(const decode_params& p, int n_tok, int group, hipStream_t stream)
 		{
@@ -728,9 +846,15 @@ namespace nnchip
 					decode_q4_multi_kernel<NB><<<dim3(p.n_split, p.n_kv, (pairs + 16 * kW - 1) / (16 * kW)), threads, 0, stream>>>(p, group);
 			if constexpr (NB <= 4)
 				if (pairs > 8 && pairs <= 16)
-					decode_q4_kernel<NB, 2><<<dim3(p.n_split, p.n_kv, 1), threads, 0, stream>>>(p, group);
+					decode_q4_kernel<NB, 2, false><<<dim3(p.n_split, p.n_kv, 1), threads, 0, stream>>>(p, group);
+			if constexpr (NB <= 8)
+				if (n_tok == 1 && pairs <= 8 && p.n_split > 1 && p.n_split <= kFuseSplits && p.counts)
+				{
+					decode_q4_kernel<NB, 1, true><<<dim3(p.n_split, p.n_kv, 1), threads, 0, stream>>>(p, group);
+					return;
+				}
 			if (pairs <= 8 || (NB > 4 && pairs <= 16) || NB > 8)
-				decode_q4_kernel<NB, 1><<<dim3(p.n_split, p.n_kv, tiles), threads, 0, stream>>>(p, group);
+				decode_q4_kernel<NB, 1, false><<<dim3(p.n_split, p.n_kv, tiles), threads, 0, stream>>>(p, group);
 			if (p.n_split > 1)
 				merge_q4_kernel<<<dim3(p.n_head, n_tok), kMergeThreads, 0, stream>>>(p, NB * kQ4Block, group);
 		}

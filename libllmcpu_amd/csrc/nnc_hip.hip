@@ -480,14 +480,17 @@ namespace
 		return static_cast<int>(sk);
 	}
 
-	// Keys per work-group of the 4-bit cache's split kernel for one token's span:
-	// about two work-groups per CU (what its registers let be resident up to
-	// head_dim 128), at most kSplitsPerGroupMax per KV head, in whole rounds of a
-	// work-group's wavefronts, or for short spans in units.
+	// Keys per work-group of the 4-bit cache's split kernel for one token's span, in
+	// whole rounds of a work-group's wavefronts: about two work-groups per CU (what
+	// its registers let be resident up to head_dim 128), at most
+	// kSplitsPerGroupMax per KV head. (In units of one wavefront, short spans on
+	// more CUs: one KV head of 256 at 1k keys, 32 splits of 32 keys and a merge
+	// launch, 6.6 us a call of three streams and 10.2 in a graph; eight of 128 that
+	// merge in the launch 4.2 and 10.0, four of 256 4.7 and 11.3.)
 	int split_keys_q4(const nnc_hip_kv* kv, int kmin, int kmax, int n_kv, int head_dim)
 	{
-		return split_keys_for(kv, kmin, kmax, head_dim <= 128 ? (n_kv + 1) / 2 : n_kv, nnchip::kQ4UnitKeys * nnchip::kQ4Waves,
-		                      nnchip::kQ4UnitKeys);
+		constexpr int round = nnchip::kQ4UnitKeys * nnchip::kQ4Waves;
+		return split_keys_for(kv, kmin, kmax, head_dim <= 128 ? (n_kv + 1) / 2 : n_kv, round, round);
 	}
 
 	// One split-K launch: tokens t0 .. t0 + n - 1 of a call on the absolute
@@ -619,7 +622,7 @@ namespace
 		p.qscale = scale * 1.4426950408889634f;
 		// One-token launches of the MFMA kernels over a few splits merge in
 		// the split launch; the counts are the cache's, used in stream order.
-		if (nnchip::mfma_shape(head_dim, group) && n_kv <= nnchip::kFuseCounts) p.counts = kv->counts;
+		if ((kv->q4 || nnchip::mfma_shape(head_dim, group)) && n_kv <= nnchip::kFuseCounts) p.counts = kv->counts;
 		if (kv->q4 ? !nnchip::launch_decode_q4(p, n_tok, head_dim, group, kv->stream)
 		           : !nnchip::launch_decode(p, n_tok, head_dim, group, kv->bf16, kv->stream))
 			return fail(NNC_ERR_UNSUPPORTED_MODEL, "no decode kernel for head_dim %d, group %d", head_dim, group);
