@@ -11,7 +11,9 @@
 //   P = 2^(S - offset) (running offset and sum per row; see kRaise)
 //   O^T += V^T P^T     (the lane's own weights are the operand: a lane's eight k
 //                       slots of a product are taken to be the keys it holds)
-// The key groups of a row meet in LDS at the end. TR is 32 (32 x 32 products) up
+// The key groups of a row meet in LDS at the end. Where few rows have many keys,
+// several work-groups share a tile's steps, and a second launch merges what they
+// wrote (flash_plan). TR is 32 (32 x 32 products) up
 // to head_dim 128, and 16 (16 x 16 products, half the rows' O and Q) at 256, so
 // that two wavefronts' registers fit on a SIMD: one's products run beside the
 // other's softmax and conversions.
@@ -32,6 +34,7 @@
 #include "kernels.h"
 #include "kv_q4.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace nnchip
@@ -46,12 +49,15 @@ namespace nnchip
 
 		constexpr int kBufferFlags = 0x00020000; // buffer descriptor word 3: raw 32-bit data
 
+		// Keys of a step: as many as leave two wavefronts' registers on a SIMD.
+		constexpr int flash_step(int mode, int hd) { return hd <= (mode == kF32 ? 96 : mode == kQ4 ? 128 : 256) ? 64 : 32; }
+
 		template <int MODE_, int HD_, int TR_, int RG_, int KG_>
 		struct shape
 		{
 			static constexpr int MODE = MODE_, HD = HD_, TR = TR_, RG = RG_, KG = KG_;
 			static constexpr int WAVES = RG * KG, ROWS = TR * RG;
-			static constexpr int KS = HD <= (MODE == kF32 ? 96 : 128) ? 64 : 32; // keys of a step
+			static constexpr int KS = flash_step(MODE, HD); // keys of a step
 			static constexpr int KP = HD + 8, VP = KS + 8; // halves per K row, per V^T row (an odd number of 16 bytes)
 			static constexpr int PARTS = MODE == kF32 ? 2 : 1; // hi, lo
 			static constexpr int K_HALVES = KS * KP, V_HALVES = HD * VP;
@@ -124,9 +130,11 @@ namespace nnchip
 
 		// A row's attention in fp32 on the vector ALUs by one wavefront, every
 		// operand straight from memory: 64 keys at a time, a lane per key for the
-		// scores and per column for the outputs.
+		// scores and per column for the outputs. part: where the row's partial goes
+		// (head_dim sums, offset, weights' sum), or null: to out.
 		template <int MODE>
-		__device__ void vector_row(const flash_params& p, size_t row_at, int tok, int head, int kvh, int first, int last, int lane)
+		__device__ void vector_row(const flash_params& p, size_t row_at, int tok, int head, int kvh, int first, int last,
+		                           int lane, float* part)
 		{
 			auto el = [](const void* b, size_t i)
 			{
@@ -164,13 +172,15 @@ namespace nnchip
 				}
 			}
 			for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
-			const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+			if (part && lane == 0) *reinterpret_cast<float2*>(part + hd) = make_float2(m, l);
+			const float inv = part ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 			const size_t oi = (row_at + tok) * p.out_stride + static_cast<size_t>(head) * hd;
 			for (int c = 0; c < kFlashMaxDim / 64; ++c)
 			{
 				const int d = 64 * c + lane;
 				if (d >= hd) continue;
-				if constexpr (MODE == kBf16) static_cast<uint16_t*>(p.out)[oi + d] = static_cast<uint16_t>(cvt_pk_bf16(o[c] * inv, 0.0f));
+				if (part) part[d] = o[c];
+				else if constexpr (MODE == kBf16) static_cast<uint16_t*>(p.out)[oi + d] = static_cast<uint16_t>(cvt_pk_bf16(o[c] * inv, 0.0f));
 				else static_cast<float*>(p.out)[oi + d] = o[c] * inv;
 			}
 		}
@@ -239,7 +249,8 @@ namespace nnchip
 			const long long n_rows = static_cast<long long>(len) * group;
 			// (the last rows of a causal sequence have the most keys: they go first)
 			const int n_blk = static_cast<int>((n_rows + G::ROWS - 1) / G::ROWS);
-			const long long r0 = static_cast<long long>(n_blk - 1 - (tile - seqs.tile[s_idx])) * G::ROWS;
+			const int n_split = seqs.split[s_idx], sp = (tile - seqs.tile[s_idx]) % n_split;
+			const long long r0 = static_cast<long long>(n_blk - 1 - (tile - seqs.tile[s_idx]) / n_split) * G::ROWS;
 			const int pos0 = MODE == kQ4 ? p.pos0 : 0, n_keys = MODE == kQ4 ? p.n_seq : len;
 
 			auto token_of = [&](long long r) { return static_cast<int>((r < n_rows ? r : n_rows - 1) / group); };
@@ -256,6 +267,14 @@ namespace nnchip
 			span_of(r0 + G::ROWS - 1, unused, kmax);
 			span_of(w0, unused, full_to); // every row of the wavefront sees full_from .. full_to
 			span_of(w0 + TR - 1, full_from, unused);
+			// The work-group's steps: its share of those from kmin's on.
+			const int k_first = kmin / KS * KS;
+			const int all_steps = kmax < k_first ? 0 : (kmax - k_first) / KS + 1;
+			const int s_from = static_cast<int>(static_cast<long long>(all_steps) * sp / n_split);
+			const int s_to = static_cast<int>(static_cast<long long>(all_steps) * (sp + 1) / n_split);
+			const int k_from = k_first + s_from * KS, k_end = k_first + s_to * KS; // (a key group may step past k_end: masked)
+			last = last < k_end - 1 ? last : k_end - 1;
+			full_to = full_to < k_end - 1 ? full_to : k_end - 1;
 
 			// ---- Q ----
 			constexpr int NQ = G::NQ;
@@ -350,7 +369,7 @@ namespace nnchip
 			// the work-group's last key none: zeros).
 			auto rows_from = [&](const void* base, size_t stride, int k0)
 			{
-				const int n = k0 > kmax ? 0 : n_keys - k0 < KS ? n_keys - k0 : KS;
+				const int n = k0 > kmax || k0 >= k_end ? 0 : n_keys - k0 < KS ? n_keys - k0 : KS;
 				const char* at = static_cast<const char*>(base) + ((row_at + k0) * stride + static_cast<size_t>(kvh) * hd) * ESIZE;
 				return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(at), 0, n ? static_cast<int>(((n - 1) * stride + hd) * ESIZE) : 0, kBufferFlags);
 			};
@@ -366,7 +385,7 @@ namespace nnchip
 						g.code[n] = u32x4{0, 0, 0, 0};
 						g.ksz[n] = u32x2{0, 0};
 						g.vs[n] = g.vz[n] = u32x4{0, 0, 0, 0};
-						if (gi >= KS / 32 || b >= blocks || k0 + 32 * gi > kmax) continue;
+						if (gi >= KS / 32 || b >= blocks || k0 + 32 * gi > kmax || k0 >= k_end) continue;
 						const unsigned char* at = static_cast<const unsigned char*>(p.k) +
 						                          (static_cast<size_t>((k0 / kQ4Rows + gi) % groups) * (p.n_kv * blocks) + kvh * blocks + b) * kQ4Record;
 						g.code[n] = *reinterpret_cast<const u32x4*>(at + 16 * lane);
@@ -522,10 +541,8 @@ namespace nnchip
 			};
 
 			regs_t regs;
-			const int k_first = kmin / KS * KS;
-			const int n_steps = kmax < k_first ? 0 : (kmax - k_first) / KS + 1;
-			if (n_steps) load_step(k_first + kg * KS, regs);
-			for (int step = kg; step - kg < n_steps; step += G::KG) // (as often for every key group)
+			if (s_from < s_to) load_step(k_from + kg * KS, regs);
+			for (int step = s_from + kg; step - kg < s_to; step += G::KG) // (as often for every key group)
 			{
 				const int k0 = k_first + step * KS;
 				// Largest magnitudes (F32), or whether V holds an infinite or NaN element
@@ -581,7 +598,7 @@ namespace nnchip
 				}
 				// (a key group past the last step stores zeros, and all its keys are masked)
 				store_step(regs, ek, ev);
-				if (step + G::KG - kg < n_steps) load_step(k0 + G::KG * KS, regs);
+				if (step + G::KG - kg < s_to) load_step(k0 + G::KG * KS, regs);
 				__syncthreads();
 
 				acc_t s[NS] = {};
@@ -658,6 +675,8 @@ namespace nnchip
 				}
 			}
 
+			auto part_of_row = [&](long long r)
+			{ return p.part + (seqs.part[s_idx] + (static_cast<size_t>(r) * p.n_kv + kvh) * n_split + sp) * (hd + 4); };
 			l = row_sum<TR>(l);
 			if constexpr (MODE == kF32)
 				if (ev_o != 1000)
@@ -674,7 +693,8 @@ namespace nnchip
 						const long long x = r0 + r;
 						int a, b;
 						span_of(x, a, b);
-						vector_row<MODE>(p, row_at, token_of(x), kvh * group + static_cast<int>(x % group), kvh, a, b, lane);
+						vector_row<MODE>(p, row_at, token_of(x), kvh * group + static_cast<int>(x % group), kvh, a > k_from ? a : k_from,
+						                 b < k_end - 1 ? b : k_end - 1, lane, n_split > 1 ? part_of_row(x) : nullptr);
 					}
 					return;
 				}
@@ -721,6 +741,20 @@ namespace nnchip
 
 			// ---- out ----
 			if (!real) return;
+			if (n_split > 1)
+			{
+				float* const part = part_of_row(row);
+#pragma unroll
+				for (int dt = 0; dt < NO; ++dt)
+#pragma unroll
+					for (int c = 0; c < EL / 4; ++c)
+					{
+						const int d = TR * dt + 8 * c + 4 * sub;
+						if (d < hd) *reinterpret_cast<float4*>(part + d) = float4{o[dt][4 * c], o[dt][4 * c + 1], o[dt][4 * c + 2], o[dt][4 * c + 3]};
+					}
+				if (sub == 0) *reinterpret_cast<float2*>(part + hd) = make_float2(off, l);
+				return;
+			}
 			const float inv = l == 0.0f ? 0.0f : 1.0f / l; // (a row that sees nothing: zeros)
 			const size_t oi = (row_at + tok) * p.out_stride + static_cast<size_t>(head) * hd;
 #pragma unroll
@@ -744,7 +778,56 @@ namespace nnchip
 				}
 		}
 
-		// Fills in the tiles of `rows` rows and launches.
+		// The partials of rows whose keys several work-groups shared, joined in key
+		// order. A float4 column of a row per thread.
+		template <int MODE, int NSEQ>
+		__global__ __launch_bounds__(256) void flash_merge_kernel(const flash_params p, const flash_seqs<NSEQ> seqs)
+		{
+			const int hd = p.head_dim, group = p.n_head / p.n_kv, cols = hd / 4, rows_here = 256 / cols;
+			const int c = threadIdx.x % cols, lane = threadIdx.x & 63;
+			int s_idx = 0;
+#pragma unroll
+			for (int x = 0; x < (NSEQ + 63) / 64; ++x)
+			{
+				const int i = 64 * x + lane;
+				s_idx += __popcll(__ballot(i < seqs.n && seqs.tile[i < NSEQ ? i : 0] <= static_cast<int>(blockIdx.x)));
+			}
+			s_idx = __builtin_amdgcn_readfirstlane(s_idx - 1);
+			const long long x = static_cast<long long>(blockIdx.x - seqs.tile[s_idx]) * rows_here + threadIdx.x / cols;
+			if (threadIdx.x / cols >= rows_here || x >= static_cast<long long>(seqs.len[s_idx]) * p.n_head) return;
+			const int n_split = seqs.split[s_idx], kvh = static_cast<int>(x % p.n_kv);
+			const long long row = x / p.n_kv;
+			const int tok = static_cast<int>(row / group), head = kvh * group + static_cast<int>(row % group);
+			const float* part = p.part + (seqs.part[s_idx] + static_cast<size_t>(x) * n_split) * (hd + 4);
+			float m = -INFINITY;
+			for (int i = 0; i < n_split; ++i) m = fmaxf(m, part[static_cast<size_t>(i) * (hd + 4) + hd]);
+			const float off = m == -INFINITY ? 0.0f : m;
+			float4 o = {0, 0, 0, 0};
+			float l = 0.0f;
+			for (int i = 0; i < n_split; ++i, part += hd + 4)
+			{
+				const float2 ml = *reinterpret_cast<const float2*>(part + hd);
+				const float4 v = *reinterpret_cast<const float4*>(part + 4 * c);
+				const float f = fast_exp2(ml.x - off);
+				o = float4{fmaf(v.x, f, o.x), fmaf(v.y, f, o.y), fmaf(v.z, f, o.z), fmaf(v.w, f, o.w)};
+				l = fmaf(ml.y, f, l);
+			}
+			const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+			float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+			const size_t at = (static_cast<size_t>(seqs.start[s_idx]) + tok) * p.out_stride + static_cast<size_t>(head) * hd + 4 * c;
+			if constexpr (MODE == kQ4)
+				for (int j = 0; j < 4; ++j) y[j] = gated(y[j], p.gate, at + j);
+			if constexpr (MODE == kBf16)
+				*reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out) + at) = u32x2{cvt_pk_bf16(y[0], y[1]), cvt_pk_bf16(y[2], y[3])};
+			else
+				*reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = float4{y[0], y[1], y[2], y[3]};
+		}
+
+		// The compiled head_dim that takes head_dim's place, and the rows of a tile.
+		int flash_dim(int hd) { return hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256; }
+		int flash_rows(int hd, int key_groups) { return flash_dim(hd) == 256 && key_groups == 2 ? 64 : 128; }
+
+		// Fills in the tiles and launches; then, where keys are shared, the merge.
 		template <class G, int NSEQ>
 		bool launch_shape(const flash_params& p, flash_seqs<NSEQ>& s, hipStream_t stream)
 		{
@@ -752,23 +835,41 @@ namespace nnchip
 			for (int i = 0; i < s.n; ++i)
 			{
 				s.tile[i] = static_cast<int>(tiles);
-				tiles += (static_cast<long long>(s.len[i]) * (p.n_head / p.n_kv) + G::ROWS - 1) / G::ROWS;
+				tiles += (static_cast<long long>(s.len[i]) * (p.n_head / p.n_kv) + G::ROWS - 1) / G::ROWS * s.split[i];
 				if (tiles * p.n_kv > 0x7fffffff) return false;
 			}
-			if (tiles)
-				flash_kernel<G, NSEQ><<<dim3(static_cast<unsigned>(tiles * p.n_kv)), 64 * G::WAVES, 0, stream>>>(p, s);
+			if (!tiles) return true;
+			flash_kernel<G, NSEQ><<<dim3(static_cast<unsigned>(tiles * p.n_kv)), 64 * G::WAVES, 0, stream>>>(p, s);
+			flash_seqs<NSEQ> m{};
+			long long groups = 0;
+			const int rows_here = 256 / (p.head_dim / 4);
+			for (int i = 0; i < s.n; ++i)
+			{
+				if (s.split[i] == 1) continue;
+				m.start[m.n] = s.start[i];
+				m.len[m.n] = s.len[i];
+				m.split[m.n] = s.split[i];
+				m.part[m.n] = s.part[i];
+				m.tile[m.n] = static_cast<int>(groups); // (partials of at most kFlashScratch bytes: few)
+				groups += (static_cast<long long>(s.len[i]) * p.n_head + rows_here - 1) / rows_here;
+				++m.n;
+			}
+			if (m.n) flash_merge_kernel<G::MODE, NSEQ><<<dim3(static_cast<unsigned>(groups)), 256, 0, stream>>>(p, m);
 			return true;
 		}
 
-		// Work-groups of `rows` rows.
-		template <int NSEQ>
-		long long work_groups(const flash_params& p, const flash_seqs<NSEQ>& s, int rows)
+		// Keys that the tile of token t0 .. reads (rows of a tile: `tokens` tokens).
+		long long tile_keys(const flash_params& p, bool q4, int len, int t0, int tokens)
 		{
-			long long n = 0;
-			for (int i = 0; i < s.n; ++i) n += (static_cast<long long>(s.len[i]) * (p.n_head / p.n_kv) + rows - 1) / rows;
-			return n * p.n_kv;
+			const int pos0 = q4 ? p.pos0 : 0, n_keys = q4 ? p.n_seq : len, t1 = std::min(t0 + tokens, len) - 1;
+			int a, b, unused;
+			attn_span(p.causal, p.window, pos0 + t0, n_keys, a, unused);
+			attn_span(p.causal, p.window, pos0 + t1, n_keys, unused, b);
+			return std::max(0, b - a + 1);
 		}
 
+		// Key groups and splits of a launch.
+		//
 		// One key group while there is a work-group for every CU; below that two, so
 		// that a CU's one work-group still has two wavefronts per SIMD (us alone /
 		// with three streams in flight, one -> two: 512 tokens of 32 over 8 x 128 at
@@ -779,36 +880,96 @@ namespace nnchip
 		// as much in flight (73 and 37). F32 at head_dim 256 converts K and V for half
 		// as many rows with two, and keeps one down to a quarter of the CUs (twelve
 		// texts of 5 to 1500 tokens of 3 x 256, 121 work-groups: 78 / 31 -> 62 / 44).
-		template <int MODE, int HD, int NSEQ>
-		bool launch_dim(const flash_params& p, flash_seqs<NSEQ>& s, int n_cu, hipStream_t stream)
+		//
+		// A sequence's keys are shared out where its longest tile has at least 2.3
+		// times the steps (64 keys) that each CU has on average, counted as 12 at least
+		// (6 where the partials are small): a launch lasts as long as its longest work-group.
+		// (us alone / three streams, not shared -> shared: 20 tokens of 4 over 1 x 256
+		// at 8k keys 282 / 95 -> 38 / 14; 40 of 32 over 8 x 128 at 6k 157 / 53 -> 39 /
+		// 18; 900 of 8 over 4 x 256 at 5k 216 / 95 -> 124 / 103.) Its partials cost
+		// memory traffic and a launch: from twice the average on, or down to 6 steps
+		// for all, what a lone stream gained others in flight lost (512 tokens at 4k
+		// keys, above, 110 / 62 -> 82 / 72; the window of 1024 52 / 26 -> 43 / 38; one
+		// BF16 prompt of 1500 tokens of 4 over 1 x 256 53 / 20 -> 41 / 29). At most
+		// `limit` bytes of partials, the longest sequences first (they come in that
+		// order).
+		constexpr double kShare = 2.3, kShareSteps = 12.0, kShareFewSteps = 6.0;
+		constexpr size_t kShareSmall = size_t{8} << 20;
+		template <int NSEQ>
+		size_t plan(const flash_params& p, flash_seqs<NSEQ>& s, int mode, int n_cu, size_t limit)
 		{
-			const bool one = work_groups(p, s, 128) > (MODE == kF32 && HD == 256 ? n_cu / 4 : n_cu);
+			const int group = p.n_head / p.n_kv, hd = flash_dim(p.head_dim);
+			long long tiles = 0;
+			for (int i = 0; i < s.n; ++i) tiles += (static_cast<long long>(s.len[i]) * group + 127) / 128;
+			s.key_groups = tiles * p.n_kv > (mode == kF32 && hd == 256 ? n_cu / 4 : n_cu) ? 1 : 2;
+			const int rows = flash_rows(hd, s.key_groups), tokens = std::max(1, rows / group);
+			auto steps_of = [&](int i, bool longest)
+			{
+				const int len = s.len[i], end = std::max(0, len - tokens);
+				const long long a = tile_keys(p, mode == kQ4, len, 0, tokens), b = tile_keys(p, mode == kQ4, len, end, tokens),
+				                mid = tile_keys(p, mode == kQ4, len, end / 2, tokens);
+				return static_cast<double>(longest ? std::max({a, b, mid}) : (a + b + 2 * mid) / 4) / 64;
+			};
+			double work = 0;
+			for (int i = 0; i < s.n; ++i)
+				work += steps_of(i, false) * static_cast<double>((static_cast<long long>(s.len[i]) * group + rows - 1) / rows) * p.n_kv;
+			size_t used = 0;
+			const size_t row_bytes = static_cast<size_t>(p.head_dim + 4) * sizeof(float);
+			for (int i = 0; i < s.n; ++i)
+			{
+				s.split[i] = 1;
+				s.part[i] = 0;
+				const double steps = steps_of(i, true);
+				const size_t one = static_cast<size_t>(s.len[i]) * p.n_head * row_bytes;
+				const bool small = one * (steps / kShareFewSteps) <= kShareSmall;
+				const double share = std::max(small ? kShareFewSteps : kShareSteps, work / n_cu);
+				if (steps < kShare * share) continue;
+				const long long fit = static_cast<long long>((limit - used) / one), want = static_cast<long long>(steps / share + 0.5);
+				const int n = static_cast<int>(std::min<long long>({fit, want, 64}));
+				if (n < 2) continue;
+				s.split[i] = n;
+				s.part[i] = static_cast<int>(used / row_bytes);
+				used += one * n;
+			}
+			return used;
+		}
+
+		template <int MODE, int HD, int NSEQ>
+		bool launch_dim(const flash_params& p, flash_seqs<NSEQ>& s, hipStream_t stream)
+		{
+			const bool one = s.key_groups == 1;
 			if constexpr (HD == 256)
 				return one ? launch_shape<shape<MODE, HD, 16, 8, 1>>(p, s, stream) : launch_shape<shape<MODE, HD, 16, 4, 2>>(p, s, stream);
 			else
 				return one ? launch_shape<shape<MODE, HD, 32, 4, 1>>(p, s, stream) : launch_shape<shape<MODE, HD, 32, 4, 2>>(p, s, stream);
 		}
-
 		template <int MODE, int NSEQ>
-		bool launch_mode(const flash_params& p, flash_seqs<NSEQ>& s, int n_cu, hipStream_t stream)
+		bool launch_mode(const flash_params& p, flash_seqs<NSEQ>& s, hipStream_t stream)
 		{
-			if (p.head_dim <= 64) return launch_dim<MODE, 64>(p, s, n_cu, stream);
-			if (p.head_dim <= 96) return launch_dim<MODE, 96>(p, s, n_cu, stream);
-			if (p.head_dim <= 128) return launch_dim<MODE, 128>(p, s, n_cu, stream);
-			return launch_dim<MODE, 256>(p, s, n_cu, stream);
+			switch (flash_dim(p.head_dim))
+			{
+			case 64: return launch_dim<MODE, 64>(p, s, stream);
+			case 96: return launch_dim<MODE, 96>(p, s, stream);
+			case 128: return launch_dim<MODE, 128>(p, s, stream);
+			default: return launch_dim<MODE, 256>(p, s, stream);
+			}
 		}
 	}
 
-	bool launch_packed(const flash_params& p, flash_seqs<kFlashSeqs>& s, bool bf16, int n_cu, hipStream_t stream)
+	size_t plan_packed(const flash_params& p, flash_seqs<kFlashSeqs>& s, bool bf16, int n_cu, size_t limit)
 	{
-		return bf16 ? launch_mode<kBf16>(p, s, n_cu, stream) : launch_mode<kF32>(p, s, n_cu, stream);
+		return plan(p, s, bf16 ? kBf16 : kF32, n_cu, limit);
 	}
-
-	bool launch_flash_q4(const flash_params& p, int n_tok, int n_cu, hipStream_t stream)
+	bool launch_packed(const flash_params& p, flash_seqs<kFlashSeqs>& s, bool bf16, hipStream_t stream)
 	{
-		flash_seqs<1> s{};
+		return bf16 ? launch_mode<kBf16>(p, s, stream) : launch_mode<kF32>(p, s, stream);
+	}
+	size_t plan_flash_q4(const flash_params& p, flash_seqs<1>& s, int n_tok, int n_cu, size_t limit)
+	{
 		s.n = 1;
+		s.start[0] = 0;
 		s.len[0] = n_tok;
-		return launch_mode<kQ4>(p, s, n_cu, stream);
+		return plan(p, s, kQ4, n_cu, limit);
 	}
+	bool launch_flash_q4(const flash_params& p, flash_seqs<1>& s, hipStream_t stream) { return launch_mode<kQ4>(p, s, stream); }
 }

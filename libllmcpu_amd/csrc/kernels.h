@@ -165,6 +165,7 @@ namespace nnchip
 		int causal, window;
 		float scale;
 		int pos0, n_seq, rows; // 4-bit: position of the first row, keys, rows of the buffer
+		float* part; // partials of shared tiles
 	};
 	constexpr int kFlashMaxDim = 256;
 	// Sequences of one launch, none of them empty: first row, length, first tile
@@ -173,12 +174,18 @@ namespace nnchip
 	template <int N>
 	struct flash_seqs
 	{
-		int n;
+		int n, key_groups;
 		int start[N], len[N], tile[N];
+		int split[N], part[N]; // work-groups that share a tile's keys, and where their partials begin (rows of head_dim + 4 floats)
 	};
-	// False, with nothing launched, for more work-groups than a grid holds.
-	bool launch_packed(const flash_params& p, flash_seqs<kFlashSeqs>& s, bool bf16, int n_cu, hipStream_t stream);
-	bool launch_flash_q4(const flash_params& p, int n_tok, int n_cu, hipStream_t stream);
+	// Key groups and splits (and the bytes of their partials, at most limit: the
+	// caller's p.part), then the launch; false, with nothing launched, for more
+	// work-groups than a grid holds.
+	constexpr size_t kFlashScratch = size_t{32} << 20;
+	size_t plan_packed(const flash_params& p, flash_seqs<kFlashSeqs>& s, bool bf16, int n_cu, size_t limit);
+	bool launch_packed(const flash_params& p, flash_seqs<kFlashSeqs>& s, bool bf16, hipStream_t stream);
+	size_t plan_flash_q4(const flash_params& p, flash_seqs<1>& s, int n_tok, int n_cu, size_t limit);
+	bool launch_flash_q4(const flash_params& p, flash_seqs<1>& s, hipStream_t stream);
 
 	// Tiled MFMA attention for a batch of query tokens.
 	struct prefill_params

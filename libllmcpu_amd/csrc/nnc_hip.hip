@@ -789,6 +789,23 @@ namespace
 		}
 	}
 
+	// Plans a launch of the tiled kernel for many rows (planned(limit): the bytes of
+	// its partials, at most limit) and finds them a place: at most kFlashScratch
+	// bytes, so that the no-alloc entry point's array holds as much and gives the
+	// same bits; while the stream is captured, what is there.
+	template <class Planned>
+	nnc_status flash_scratch(nnc_hip_kv* kv, const part_source& src, Planned planned, float*& part)
+	{
+		static_assert(nnchip::kFlashScratch <= NNC_HIP_NOALLOC_SCRATCH_BYTES, "the no-alloc array");
+		size_t bytes = planned(nnchip::kFlashScratch);
+		part = src.ptr;
+		if (src.ptr || !bytes) return NNC_OK;
+		if (bytes > kv->part.bytes && capturing(kv)) bytes = planned(kv->part.bytes);
+		else if (nnc_status s = reserve(kv, kv->part, bytes, "attention scratch")) return s;
+		part = static_cast<float*>(kv->part.ptr);
+		return NNC_OK;
+	}
+
 	nnc_status attend_impl(nnc_hip_kv* kv, int32_t buf, const float* q, float* out, const float* gate, int32_t n_tok, int32_t pos0,
 	                       int32_t n_seq, int32_t window, bool causal, int32_t n_head, int32_t n_kv, int32_t head_dim,
 	                       float scale, const part_source& src = part_source{})
@@ -826,7 +843,10 @@ namespace
 			p.pos0 = pos0;
 			p.n_seq = n_seq;
 			p.rows = b.rows;
-			if (!nnchip::launch_flash_q4(p, n_tok, kv->n_cu, kv->stream))
+			nnchip::flash_seqs<1> s{};
+			auto planned = [&](size_t limit) { return nnchip::plan_flash_q4(p, s, n_tok, kv->n_cu, limit); };
+			if (nnc_status st = flash_scratch(kv, src, planned, p.part)) return st;
+			if (!nnchip::launch_flash_q4(p, s, kv->stream))
 				return fail(NNC_ERR_UNSUPPORTED_MODEL, "%d tokens of %d heads are too many for one call", n_tok, n_head);
 			NNC_HIP_TRY(hipGetLastError(), "attention over a 4-bit cache");
 			return NNC_OK;
@@ -1430,7 +1450,9 @@ nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void
 			s.start[s.n] = starts[order[i]];
 			s.len[s.n] = starts[order[i] + 1] - starts[order[i]];
 		}
-		if (!nnchip::launch_packed(p, s, type == NNC_HIP_BF16, kv->n_cu, kv->stream))
+		auto planned = [&](size_t limit) { return nnchip::plan_packed(p, s, type == NNC_HIP_BF16, kv->n_cu, limit); };
+		if (nnc_status st = flash_scratch(kv, part_source{}, planned, p.part)) return st;
+		if (!nnchip::launch_packed(p, s, type == NNC_HIP_BF16, kv->stream))
 			return fail(NNC_ERR_UNSUPPORTED_MODEL, "too many row blocks for one launch");
 		NNC_HIP_TRY(hipGetLastError(), "packed attention");
 	}
