@@ -326,8 +326,10 @@ enum
  * head_dim a multiple of 8 up to 256, any group n_head / n_kv. F32: the error
  * of fp32 sums; BF16: weights rounded to BF16, sums in fp32, rounded once to
  * out. An infinite or NaN element of a key reaches only the rows that attend
- * it. `kv` is the execution context; queued on its stream, nothing is
- * allocated, and the call may be captured (the starts are then the graph's).
+ * it. `kv` is the execution context: queued on its stream; long sequences of
+ * few heads use its scratch (at most 32 MiB). The call may be captured (the
+ * starts are then the graph's); while the scratch has not grown yet, it takes a
+ * way that needs none (same tolerance, other bits).
  * NNC_ERR_INVALID_ARGUMENT: NULL pointers, an unknown type, starts that
  * decrease or are negative, n_head not a multiple of n_kv, pointers not
  * 16-byte aligned, strides below the row, not whole 16 bytes, or of 2^23

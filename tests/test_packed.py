@@ -276,3 +276,55 @@ def test_prompts_then_decode_over_four_bits():
     finally:
         for kv in caches:
             kv.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [True, False])
+def test_long_sequence_of_few_heads(bf16):
+    """One whose keys work-groups share, beside short ones: plain, with an infinite
+    and a NaN value in the middle of it, and captured before and after the scratch
+    for it is there."""
+    n_head, n_kv, hd = 2, 1, 64
+    starts = [0, 5, 1905, 1905, 1950]
+    shape = dict(n_head=n_head, n_kv=n_kv, head_dim=hd, scale=0.125, window=0, causal=True)
+    (q, q64), (k, k64), (v, v64) = (typed(rows_of(s, 1950, h * hd), bf16) for s, h in ((1, n_head), (2, n_kv), (3, n_kv)))
+    want, bound = expected(q64, k64, v64, starts, bf16, **shape)
+    dev = [hip_rt.malloc(x.nbytes) for x in (q, k, v, q)]
+    try:
+        with nh.KVCache([32], [32]) as kv:
+            for d, x in zip(dev, (q, k, v)):
+                hip_rt.to_device(d, x)
+
+            def call():
+                kv.attend_packed_device(*dev, starts=starts, bf16=bf16, **shape)
+
+            def out():
+                kv.sync()
+                return hip_rt.to_host(np.empty_like(q), dev[3])
+
+            early = hip_rt.Graph(kv.stream, call)
+            early.launch(kv.stream)
+            assert (np.abs(as_values(out()) - want) <= bound).all()
+            call()
+            got = out()
+            assert (np.abs(as_values(got) - want) <= bound).all()
+            late = hip_rt.Graph(kv.stream, call)
+            for _ in range(3):
+                late.launch(kv.stream)
+                assert np.array_equal(out(), got)
+                kv.attend_packed(q[:300], k[:300], v[:300], starts=[0, 300], **shape)
+            for key, value in ((900, np.inf), (1700, np.nan)):
+                x = as_values(v).astype(np.float32)
+                x[5 + key, 7] = value
+                hip_rt.to_device(dev[2], typed(x, bf16)[0])
+                call()
+                y = as_values(out())
+                hit = np.zeros(want.shape, bool)
+                hit[5 + key:1905, 7::hd] = True
+                assert (np.isnan(y[hit]) if np.isnan(value) else y[hit] == np.inf).all()
+                assert (np.abs(y - want) <= bound)[~hit].all()
+            early.close()
+            late.close()
+    finally:
+        for d in dev:
+            hip_rt.free(d)

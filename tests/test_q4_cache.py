@@ -353,3 +353,64 @@ def test_two_caches_at_once():
             kv.close()
         for d in dev:
             hip_rt.free(d)
+
+
+# ---- few tokens over many keys: their keys shared among work-groups ---------------------
+
+SHARED = [  # n_head, n_kv, head_dim, rows, n_seq, pos0, n_tok, window, causal
+    (4, 1, 256, 4096, 4000, 3980, 20, 0, True),
+    (32, 8, 128, 2560, 2500, 2460, 40, 0, True),
+    (14, 2, 64, 2048, 1901, 1871, 30, 0, True),
+    (6, 2, 96, 2304, 6000, 5950, 50, 2100, True),  # a wrapped ring
+    (3, 1, 192, 2048, 2000, 100, 25, 0, False),
+    (2, 1, 32, 4096, 3333, 3300, 17, 3001, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_head,n_kv,hd,rows,n_seq,pos0,n_tok,window,causal", SHARED)
+def test_few_tokens_over_many_keys(n_head, n_kv, hd, rows, n_seq, pos0, n_tok, window, causal):
+    """Against 64 bits, gated too; the entry point that allocates nothing and a
+    graph captured after the first call give the same bits, one captured before
+    it is within the same bound."""
+    print(f"few over many {n_head}/{n_kv}/{hd} rows {rows} n_seq {n_seq} tokens {pos0}+{n_tok} window {window}", flush=True)
+    shape = dict(window=window, causal=causal, n_head=n_head, n_kv=n_kv, head_dim=hd, scale=hd**-0.5)
+    q, gate = rows_of(9, n_tok, n_head * hd), rows_of(10, n_tok, n_head * hd)
+    kv, k, v = filled(n_seq, n_kv * hd, rows)
+    want, bound, _ = ref.attend(q, k, v, pos0=pos0, n_seq=n_seq, **shape)
+    dq, do = hip_rt.malloc(q.nbytes), hip_rt.malloc(q.nbytes)
+    try:
+        with kv:
+            hip_rt.to_device(dq, q)
+
+            def call(noalloc=False):
+                f = kv.attend_device_noalloc if noalloc else kv.attend_device
+                f(0, dq, do, n_tok=n_tok, pos0=pos0, n_seq=n_seq, **shape)
+
+            def out():
+                kv.sync()
+                return hip_rt.to_host(np.empty_like(q), do)
+
+            early = hip_rt.Graph(kv.stream, call)
+            early.launch(kv.stream)
+            assert (np.abs(out() - want) <= bound).all()
+            call()
+            got = out()
+            assert (np.abs(got - want) <= bound).all()
+            late = hip_rt.Graph(kv.stream, call)
+            for _ in range(3):
+                late.launch(kv.stream)
+                assert np.array_equal(out(), got)
+                kv.attend(0, q[:1], pos0=pos0, n_seq=n_seq, **shape)
+                early.launch(kv.stream)
+                assert (np.abs(out() - want) <= bound).all()
+            call(noalloc=True)
+            assert np.array_equal(out(), got)
+            gated = kv.attend(0, q, pos0=pos0, n_seq=n_seq, gate=gate, **shape)
+            early.close()
+            late.close()
+    finally:
+        hip_rt.free(dq)
+        hip_rt.free(do)
+    sig = 1 / (1 + np.exp(-gate.astype(np.float64)))
+    assert (np.abs(gated - want * sig) <= bound * sig + 2.0**-21 * np.abs(want)).all()
