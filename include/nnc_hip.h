@@ -105,9 +105,10 @@ nnc_status nnc_hip_kv_create(int32_t n_buf, const int32_t* rows, const int32_t* 
  * block (reference nn_ops.h:138-142) along the head: with lo and hi its least
  * and largest element,
  *   s = f16((hi - lo) * r), z = f16(lo), c = rint((x - z) / s) in 0 .. 15
- * (0 where s is 0; r is 1 / 15 in F32, all of it in F32), and x is held as f16(c * s + z), rounded once. Elements
- * are brought within +-65280 first and a NaN is held as 0, so every value of
- * such a cache is finite. The other calls take it as they take the others:
+ * (0 where s is 0; r is 1 / 15 in F32, all of it in F32), and x is held as
+ * f16(c * s + z), rounded once. Elements are brought within +-65280 first and a
+ * NaN is held as 0, so every value of such a cache is finite. The other calls
+ * take it as they take the others:
  *   nnc_hip_kv_append_f32, _f32_device and nnc_hip_kv_prep_append_device
  *     quantise on the device (rows in device memory 16-byte aligned);
  *   nnc_hip_kv_append and nnc_hip_kv_read move rows in an interchange form:
@@ -118,8 +119,9 @@ nnc_status nnc_hip_kv_create(int32_t n_buf, const int32_t* rows, const int32_t* 
  *   the attend calls compute over the values that the cache holds, with the
  *     error of fp32 sums; head_dim 32, 64, 96, 128, 192, 256 or 512 (else
  *     NNC_ERR_UNSUPPORTED_MODEL), any group up to 16. No limit on a buffer's
- *     bytes. Batches of up to 16 tokens, and every batch in exact mode, give
- *     each token the bits of its one-token call, as over the other caches.
+ *     bytes; positions, n_seq and windows up to 2^30. Batches of up to 16
+ *     tokens, and every batch in exact mode, give each token the bits of its
+ *     one-token call, as over the other caches.
  * NNC_ERR_INVALID_ARGUMENT also for rows or kv_dim that are no multiples of
  * 32 (round n_ctx up; rings are multiples of 256). */
 nnc_status nnc_hip_kv_create_q4(int32_t n_buf, const int32_t* rows, const int32_t* kv_dim, nnc_hip_kv** out);
@@ -322,9 +324,10 @@ enum
  *   q, out [rows][n_head * head_dim], k, v [rows][n_kv * head_dim]: device
  *     memory, elements of `type` (NNC_HIP_F32 or NNC_HIP_BF16 bit patterns),
  *     rows *_stride elements apart, so the four may be columns of one buffer;
- *     out may be q.
+ *     out may be q (of the same stride).
  * head_dim a multiple of 8 up to 256, any group n_head / n_kv. F32: the error
- * of fp32 sums; BF16: weights rounded to BF16, sums in fp32, rounded once to
+ * of fp32 sums, K and V taken to 22 bits and to 2^-39 of the largest element of
+ * 64 neighbouring keys (K) or of the sequence (V); BF16: weights rounded to BF16, sums in fp32, rounded once to
  * out. An infinite or NaN element of a key reaches only the rows that attend
  * it. `kv` is the execution context: queued on its stream; long sequences of
  * few heads use its scratch (at most 32 MiB). The call may be captured (the
@@ -333,8 +336,9 @@ enum
  * NNC_ERR_INVALID_ARGUMENT: NULL pointers, an unknown type, starts that
  * decrease or are negative, n_head not a multiple of n_kv, pointers not
  * 16-byte aligned, strides below the row, not whole 16 bytes, or of 2^23
- * elements and more.
- * NNC_ERR_UNSUPPORTED_MODEL: another head_dim. */
+ * elements and more, out one of k and v.
+ * NNC_ERR_UNSUPPORTED_MODEL: another head_dim, or a sequence of more than 2^28
+ * (row, head) pairs (each KV head's rounded up to 64). Nothing is written then. */
 nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void* q, size_t q_stride, const void* k,
                                         size_t k_stride, const void* v, size_t v_stride, void* out, size_t out_stride,
                                         const int32_t* starts, int32_t n_seqs, int32_t window, bool causal, int32_t n_head,

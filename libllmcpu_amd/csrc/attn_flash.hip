@@ -19,8 +19,8 @@
 // other's softmax and conversions.
 // One pass over the keys; only steps that cross a row's span are masked.
 //
-// Precision. BF16: the operands are exact, P is rounded to BF16 (2^-9 of a
-// weight; the output is rounded to BF16 as well). F32 and the 4-bit cache, whose
+// Precision. BF16: the operands are exact, P is rounded to BF16 (2^-8 of a
+// weight at most; the output is rounded to BF16 as well). F32 and the 4-bit cache, whose
 // outputs are F32: Q, P and F32's K and V are fp16 hi + lo (22 bits), brought
 // into fp16's range by powers of two (per row of Q, per step for K, running for
 // V), the product of two lo parts left out: 3 products for F32, 2 over the 4-bit
@@ -70,7 +70,7 @@ namespace nnchip
 			static constexpr int NR = (KS / 32 * (HD / 32) + RG - 1) / RG; // records per wavefront
 			static constexpr int NS = KS / TR, NO = HD / TR, EL = TR * TR / 64; // score tiles, output tiles, registers of one
 			static constexpr int QD = 512 / TR, NQ = HD / QD; // columns of a product, products over head_dim
-						static_assert(NK * THREADS * 8 == KS * HD && BYTES <= 160 << 10, "shape");
+		static_assert(NK * THREADS * 8 == KS * HD && BYTES <= 160 << 10, "shape");
 		};
 
 		// What a step's loads leave in registers until LDS is free.
@@ -836,7 +836,7 @@ namespace nnchip
 			{
 				s.tile[i] = static_cast<int>(tiles);
 				tiles += (static_cast<long long>(s.len[i]) * (p.n_head / p.n_kv) + G::ROWS - 1) / G::ROWS * s.split[i];
-				if (tiles * p.n_kv > 0x7fffffff) return false;
+				if (tiles * p.n_kv * (64 * G::WAVES) > 0xffffffffll) return false;
 			}
 			if (!tiles) return true;
 			flash_kernel<G, NSEQ><<<dim3(static_cast<unsigned>(tiles * p.n_kv)), 64 * G::WAVES, 0, stream>>>(p, s);

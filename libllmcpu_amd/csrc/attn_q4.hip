@@ -12,7 +12,7 @@
 // alone.
 //
 // A work-group of four wavefronts owns one KV head, one range of keys and T
-// columns tiles of 8 pairs; its wavefronts take groups of 32 keys in turn
+// tiles of 8 pairs; its wavefronts take groups of 32 keys in turn
 // (record by record, straight into operand registers), keep running maxima and
 // sums of their own, and meet in LDS at the end.
 #include "kernels.h"

@@ -919,6 +919,8 @@ namespace
 		return NNC_OK;
 	}
 
+	constexpr int kQ4Positions = 1 << 30; // (a step past the last key, and span ends, stay in an int)
+
 	nnc_status check_attend(const nnc_hip_kv* kv, int32_t buf, const float* q, const float* out, int32_t n_tok,
 	                        int32_t pos0, int32_t n_seq, int32_t window, bool causal, int32_t n_head, int32_t n_kv,
 	                        int32_t head_dim)
@@ -944,6 +946,9 @@ namespace
 		if (kv->q4 && !nnchip::q4_head_dim(head_dim))
 			return fail(NNC_ERR_UNSUPPORTED_MODEL,
 			            "head_dim %d is not supported over a 4-bit cache (32, 64, 96, 128, 192, 256 or 512)", head_dim);
+		if (kv->q4 && (n_seq > kQ4Positions || static_cast<long long>(pos0) + n_tok > kQ4Positions || window > kQ4Positions))
+			return fail(NNC_ERR_INVALID_ARGUMENT, "positions up to %lld, n_seq %d, window %d: past 2^30",
+			            static_cast<long long>(pos0) + n_tok, n_seq, window);
 		if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15)
 			return fail(NNC_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
 		// The BF16 kernels address a buffer with 32-bit byte offsets.
@@ -1402,9 +1407,18 @@ nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void
 		return fail(NNC_ERR_INVALID_ARGUMENT,
 		            "row strides %zu, %zu, %zu, %zu: at least the row's %zu or %zu elements, multiples of %zu, under %zu", q_stride,
 		            k_stride, v_stride, out_stride, q_dim, kv_dim, step, most);
+	if (out == k || out == v || (out == q && out_stride != q_stride))
+		return fail(NNC_ERR_INVALID_ARGUMENT, "out may be q with q's stride, and no other operand");
+	// 64-row blocks of a sequence at most (a launch holds 2^32 threads, 512 to a block).
+	const long long most_blocks = 1ll << 22;
+	auto blocks_of = [&](int32_t i)
+	{ return (static_cast<long long>(starts[i + 1] - starts[i]) * (n_head / n_kv) + 63) / 64 * n_kv; };
 	for (int32_t i = 0; i < n_seqs; ++i)
 		if (starts[0] < 0 || starts[i + 1] < starts[i])
 			return fail(NNC_ERR_INVALID_ARGUMENT, "sequence %d: rows %d up to %d", i, starts[i], starts[i + 1]);
+		else if (blocks_of(i) > most_blocks)
+			return fail(NNC_ERR_UNSUPPORTED_MODEL, "sequence %d: %d rows of %d heads are too many for one call", i,
+			            starts[i + 1] - starts[i], n_head);
 
 	// The longest first, kFlashSeqs to a launch, so that no long tile is begun
 	// last.
@@ -1439,21 +1453,20 @@ nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void
 	p.causal = causal ? 1 : 0;
 	p.window = window;
 	p.scale = scale;
-	// (rows of 2^31 tokens and 2^31 work-groups need terabytes of q: no call that
-	// fits the device is refused after a launch)
 	const device_scope on(kv->device);
-	for (size_t at = 0; at < order.size(); at += nnchip::kFlashSeqs)
+	for (size_t at = 0; at < order.size();)
 	{
 		nnchip::flash_seqs<nnchip::kFlashSeqs> s{};
-		for (size_t i = at; i < std::min(at + nnchip::kFlashSeqs, order.size()); ++i, ++s.n)
+		for (long long blocks = 0; at < order.size() && s.n < nnchip::kFlashSeqs; ++at, ++s.n)
 		{
-			s.start[s.n] = starts[order[i]];
-			s.len[s.n] = starts[order[i] + 1] - starts[order[i]];
+			if ((blocks += blocks_of(order[at])) > most_blocks) break;
+			s.start[s.n] = starts[order[at]];
+			s.len[s.n] = starts[order[at] + 1] - starts[order[at]];
 		}
 		auto planned = [&](size_t limit) { return nnchip::plan_packed(p, s, type == NNC_HIP_BF16, kv->n_cu, limit); };
 		if (nnc_status st = flash_scratch(kv, part_source{}, planned, p.part)) return st;
 		if (!nnchip::launch_packed(p, s, type == NNC_HIP_BF16, kv->stream))
-			return fail(NNC_ERR_UNSUPPORTED_MODEL, "too many row blocks for one launch");
+			return fail(NNC_ERR_UNSUPPORTED_MODEL, "too many row blocks for one launch"); // (not with most_blocks)
 		NNC_HIP_TRY(hipGetLastError(), "packed attention");
 	}
 	return NNC_OK;

@@ -328,3 +328,56 @@ def test_long_sequence_of_few_heads(bf16):
     finally:
         for d in dev:
             hip_rt.free(d)
+
+
+@pytest.mark.gpu
+def test_more_refusals():
+    """Operands that out may not be, and sequences past a launch (no memory behind the
+    addresses: refused before anything is queued)."""
+    with nh.KVCache([32], [32]) as kv:
+        ok = dict(starts=[0, 0], bf16=True, n_head=4, n_kv=2, head_dim=64, scale=0.1)
+        q, k, v = 1 << 20, 2 << 20, 3 << 20
+        kv.attend_packed_device(q, k, v, q, **ok)
+        kv.attend_packed_device(q, k, k, q, q_stride=1024, out_stride=1024, **ok)
+        for out, more in ((k, {}), (v, {}), (q, dict(q_stride=512)), (q, dict(out_stride=264))):
+            with pytest.raises(nh.NncError) as e:
+                kv.attend_packed_device(q, k, v, out, **{**ok, **more})
+            assert e.value.status == nh.NncStatus.INVALID_ARGUMENT
+        with pytest.raises(nh.NncError) as e:
+            kv.attend_packed_device(q, k, v, 4 << 20, **{**ok, "starts": [0, 1, 1 + 2**26 + 1]})
+        assert e.value.status == nh.NncStatus.UNSUPPORTED_MODEL
+        x = rows_of(1, 8, 64)
+        for starts, short in (([0, 9], 0), ([0, 8], 1), ([0, 8], 2), ([9, 9], 0)):
+            a = [x, x, x]
+            a[short] = a[short][:7] if starts[1] == 8 else x
+            with pytest.raises(ValueError):
+                kv.attend_packed(*a, starts=starts, n_head=1, n_kv=1, head_dim=64, scale=0.1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_largest_stride_and_offsets_past_32_bits(bf16, hd):
+    """Rows as far apart as the entry point takes, from a row on whose offset passes
+    2^32 bytes."""
+    n, at, es = 70, 300 if bf16 else 150, 2 if bf16 else 4
+    stride = (1 << 23) - 8
+    shape = dict(n_head=2, n_kv=1, head_dim=hd, scale=hd**-0.5, window=0, causal=True)
+    (q, q64), (k, k64), (v, v64) = (typed(rows_of(s, n, h * hd), bf16) for s, h in ((1, 2), (2, 1), (3, 1)))
+    want, bound = expected(q64, k64, v64, [0, n], bf16, **shape)
+    assert at * stride * es > 1 << 32
+    print(f"largest stride, head_dim {hd}, bf16 {bf16}", flush=True)
+    base = hip_rt.malloc((at + n) * stride * es)
+    try:
+        where = [base, base + 2 * hd * es, base + 3 * hd * es, base + 4 * hd * es]  # q, k, v, out
+        for p, x in zip(where, (q, k, v)):
+            for i in range(n):
+                hip_rt.to_device(p + (at + i) * stride * es, x[i])
+        with nh.KVCache([32], [32]) as kv:
+            kv.attend_packed_device(*where, starts=[at, at + n], bf16=bf16, q_stride=stride, k_stride=stride, v_stride=stride,
+                                    out_stride=stride, **shape)
+            kv.sync()
+        got = np.stack([hip_rt.to_host(np.empty_like(q[0]), where[3] + (at + i) * stride * es) for i in range(n)])
+    finally:
+        hip_rt.free(base)
+    assert (np.abs(as_values(got) - want) <= bound).all()

@@ -414,3 +414,21 @@ def test_few_tokens_over_many_keys(n_head, n_kv, hd, rows, n_seq, pos0, n_tok, w
         hip_rt.free(do)
     sig = 1 / (1 + np.exp(-gate.astype(np.float64)))
     assert (np.abs(gated - want * sig) <= bound * sig + 2.0**-21 * np.abs(want)).all()
+
+
+@pytest.mark.gpu
+def test_positions_past_the_limit():
+    """Rings keep any position up to 2^30; past it the attend calls refuse."""
+    far = (1 << 30) - 40
+    shape = dict(window=100, causal=True, n_head=2, n_kv=1, head_dim=64, scale=0.125)
+    k, v, q = rows_of(1, 256, 64), rows_of(2, 256, 64), rows_of(3, 30, 128)
+    with nh.KVCache([256], [64], q4=True) as kv:
+        kv.append_f32(0, far - 226, k, v)  # positions far - 226 .. far + 29
+        for n in (30, 3, 1):
+            got = kv.attend(0, q[:n], pos0=far + 30 - n, n_seq=far + 30, **shape)
+            want, bound, _ = ref.attend(q[:n], ref.values(ref.quantise(k)), ref.values(ref.quantise(v)), pos0=256 - n, n_seq=256, **shape)
+            assert (np.abs(got - want) <= bound).all()
+        for bad in (dict(pos0=far + 30), dict(pos0=far, n_seq=(1 << 30) + 1), dict(pos0=2**31 - 31), dict(pos0=far, window=2**31 - 1, causal=False)):
+            with pytest.raises(nh.NncError) as e:
+                kv.attend(0, q, **{**shape, "n_seq": far + 30, **bad})
+            assert e.value.status == nh.NncStatus.INVALID_ARGUMENT
