@@ -13,18 +13,27 @@
 //                       slots of a product are taken to be the keys it holds)
 // The key groups of a row meet in LDS at the end. Where few rows have many keys,
 // several work-groups share a tile's steps, and a second launch merges what they
-// wrote (flash_plan). TR is 32 (32 x 32 products) up
-// to head_dim 128, and 16 (16 x 16 products, half the rows' O and Q) at 256, so
-// that two wavefronts' registers fit on a SIMD: one's products run beside the
-// other's softmax and conversions.
+// wrote (plan). TR is 32 (32 x 32 products) up to head_dim 128, and 16 (16 x 16
+// products, half the rows' O and Q) at 256, so that two wavefronts' registers fit
+// on a SIMD: one's products run beside the other's softmax and conversions.
 // One pass over the keys; only steps that cross a row's span are masked.
 //
 // Precision. BF16: the operands are exact, P is rounded to BF16 (2^-8 of a
-// weight at most; the output is rounded to BF16 as well). F32 and the 4-bit cache, whose
-// outputs are F32: Q, P and F32's K and V are fp16 hi + lo (22 bits), brought
-// into fp16's range by powers of two (per row of Q, per step for K, running for
-// V), the product of two lo parts left out: 3 products for F32, 2 over the 4-bit
-// cache, whose values are fp16 themselves. Scores, sums and outputs are fp32.
+// weight at most; the output is rounded to BF16 as well). F32 and the 4-bit
+// cache, whose outputs are F32: Q, P and F32's K and V are fp16 hi + lo (22 bits),
+// brought into fp16's range by powers of two (per row of Q, per step for K,
+// running for V), the product of two lo parts left out: 3 products for F32, 2
+// over the 4-bit cache, whose values are fp16 themselves. Scores, sums and
+// outputs are fp32.
+//
+// Bound: the matrix cores' products beside the softmax's and the conversions'
+// VALU work, which two wavefronts per SIMD overlap in part. Useful flops (masked
+// ones not counted), where a large BF16 product reaches 1235 TFLOP/s: 8192 tokens
+// of 32 over 8 x 64 in BF16 870, eight prompts of 1 to 2048 of 32 over 8 x 128 740,
+// 512 tokens over 4096 keys in 4 bits (two products for one) 520 with three
+// streams. Tried without gain: two sets of tiles and one barrier a step (2-8 %
+// slower up to head_dim 128, 2 % faster at 256), wave priorities around the
+// products or the softmax, 16 rows and four wavefronts per SIMD.
 //
 // Elements that are infinite or NaN: a key's reach only the rows that attend it.
 // Scores of masked keys are replaced, but 0 x inf in P V is not, and inf has no

@@ -15,6 +15,13 @@
 // tiles of 8 pairs; its wavefronts take groups of 32 keys in turn
 // (record by record, straight into operand registers), keep running maxima and
 // sums of their own, and meet in LDS at the end.
+//
+// Bound: HBM for long spans (five bits an element, K and V once: 32 768 keys of 8 x
+// 128, 42 MB, 10.5 us a call of three streams; 131 072 of 8 x 64, 84 MB, 17.7:
+// 4.0 and 4.7 TB/s, a large copy's rate is 4.76), beside the VALU work that makes
+// fp16 of the codes (13 operations for eight); the launch and its chain of loads,
+// softmax and merge for short ones (1024 keys of one head of 256: 9.8 us alone,
+// 5.0 in flight, of which the host's call is 4.1).
 #include "kernels.h"
 #include "kv_q4.h"
 
@@ -549,9 +556,12 @@ namespace nnchip
 		// into operands in LDS while they compute on the group before. The classes
 		// that decode_q4_kernel's wavefronts are (groups by their number in the split
 		// modulo kW) follow one another, with sums of their own, and join in the same
-		// order, so a pair gets the same bits. (With the kernel above, two tiles of 8
-		// pairs per wavefront, every tile's weights computed twice and every value
-		// made four times: 13 tokens of 32 over 8 x 128 at 20k keys 68 us a call.)
+		// order, so a pair gets the same bits. Bound: VALU (the softmax of 16 pairs in
+		// fp16 parts, and every class's sums joined: some 300 operations per group of 32
+		// keys; matrix units 17 % busy) and the partials, as many bytes as the records.
+		// (13 tokens of 32 over 8 x 128 at 20k keys: 21.3 us a call; with the kernel
+		// above, two tiles of 8 pairs per wavefront, every tile's weights computed twice
+		// and every value made four times, 68.)
 		template <int NB>
 		__global__ __launch_bounds__(64 * kW, NB <= 4 ? 2 : 1) void decode_q4_multi_kernel(const decode_params p, int group)
 		{

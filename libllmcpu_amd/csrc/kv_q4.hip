@@ -88,8 +88,10 @@ namespace nnchip
 		// and its last positions. K's words belong to one row each; V's hold eight
 		// rows, so a group of which only some rows are written keeps the others'
 		// nibbles. One wavefront writes a record, so nothing else does meanwhile.
-		// Bound: HBM (4 bytes an element read, 0.625 written); one row: a load, the
-		// quotients and a store, one after the other.
+		// Bound: HBM (4 bytes an element read, 0.625 written: 4096 rows of 1024, 38.8 MB
+		// in 11.3 us, 3.4 TB/s, the read of their values 9); one row: a load, the
+		// quotients and a store, one after the other (6 us; with the old nibbles loaded
+		// ahead of the quotients 0.5 more).
 		template <bool RAW>
 		__global__ __launch_bounds__(64 * kWaves) void append_q4_kernel(unsigned char* recs, const void* k_rows,
 		                                                                const void* v_rows, int rows, int kv_dim, int pos0,
