@@ -911,24 +911,24 @@ namespace nnchip
 		// One key group while there is a work-group for every CU; below that two, so
 		// that a CU's one work-group still has two wavefronts per SIMD (us alone /
 		// with three streams in flight, one -> two: 512 tokens of 32 over 8 x 128 at
-		// 4k keys over 4 bits, 128 work-groups, 133 / 59.6 -> 104 / 58.4; 1024 of 8
-		// over 4 x 256, a window of 1024, 64 work-groups, 73 / 25.1 -> 48 / 23.0;
+		// 4k keys over 4 bits, 128 work-groups, 137 / 65 -> 108 / 61; 1024 of 8
+		// over 4 x 256, a window of 1024, 64 work-groups, 72 / 25 -> 48 / 25;
 		// eight prompts of 1 to 2048 tokens, 1752 work-groups, 113 / 113 -> 152 /
 		// 148). Four key groups of half the rows gain more alone (78 and 38) and lose
 		// as much in flight (73 and 37). F32 at head_dim 256 converts K and V for half
 		// as many rows with two, and keeps one down to a quarter of the CUs (twelve
-		// texts of 5 to 1500 tokens of 3 x 256, 121 work-groups: 78 / 31 -> 62 / 44).
+		// texts of 5 to 1500 tokens of 3 x 256, 121 work-groups: 77 / 33 -> 63 / 44).
 		//
 		// A sequence's keys are shared out where its longest tile has at least 2.3
 		// times the steps (64 keys) that each CU has on average, counted as 12 at least
 		// (6 where the partials are small): a launch lasts as long as its longest work-group.
 		// (us alone / three streams, not shared -> shared: 20 tokens of 4 over 1 x 256
-		// at 8k keys 282 / 95 -> 38 / 14; 40 of 32 over 8 x 128 at 6k 157 / 53 -> 39 /
-		// 18; 900 of 8 over 4 x 256 at 5k 216 / 95 -> 124 / 103.) Its partials cost
+		// at 8k keys 265 / 90 -> 37 / 14; 40 of 32 over 8 x 128 at 6k 154 / 52 -> 39 /
+		// 18; 900 of 8 over 4 x 256 at 5k 203 / 89 -> 116 / 95.) Its partials cost
 		// memory traffic and a launch: from twice the average on, or down to 6 steps
 		// for all, what a lone stream gained others in flight lost (512 tokens at 4k
-		// keys, above, 110 / 62 -> 82 / 72; the window of 1024 52 / 26 -> 43 / 38; one
-		// BF16 prompt of 1500 tokens of 4 over 1 x 256 53 / 20 -> 41 / 29). At most
+		// keys, above, 108 / 61 -> 80 / 72; the window of 1024 48 / 25 -> 42 / 32; one
+		// BF16 prompt of 1500 tokens of 4 over 1 x 256 51 / 18 -> 39 / 27). At most
 		// `limit` bytes of partials, the longest sequences first (they come in that
 		// order).
 		constexpr double kShare = 2.3, kShareSteps = 12.0, kShareFewSteps = 6.0;
