@@ -381,3 +381,64 @@ def test_largest_stride_and_offsets_past_32_bits(bf16, hd):
     finally:
         hip_rt.free(base)
     assert (np.abs(as_values(got) - want) <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [True, False])
+@pytest.mark.parametrize("n_head,n_kv,hd,window,causal,lens", [
+    (2, 1, 64, 0, True, [3000, 4, 2500, 0, 2000, 700]),  # several sequences share their keys in one launch
+    (1, 1, 256, 0, False, [1500, 1501]),
+    (64, 1, 16, 0, True, [130]),
+    (33, 33, 8, 1, True, [70, 1]),
+    (3, 1, 128, 1000, False, [40, 900]),
+    (4, 2, 248, 3, False, [100] * 3),
+    (2, 2, 40, 0, True, [64] * 70),
+])
+def test_corners(n_head, n_kv, hd, window, causal, lens, bf16):
+    print(f"packed corner {n_head}/{n_kv}/{hd} window {window} causal {causal} bf16 {bf16} {len(lens)} sequences", flush=True)
+    starts = [0, *np.cumsum(lens).tolist()]
+    shape = dict(window=window, causal=causal, n_head=n_head, n_kv=n_kv, head_dim=hd, scale=hd**-0.5)
+    (q, q64), (k, k64), (v, v64) = (typed(rows_of(s, starts[-1], h * hd), bf16) for s, h in ((1, n_head), (2, n_kv), (3, n_kv)))
+    with nh.KVCache([32], [32]) as kv:
+        got = kv.attend_packed(q, k, v, starts=starts, **shape)
+    want, bound = expected(q64, k64, v64, starts, bf16, **shape)
+    assert (np.abs(as_values(got) - want) <= bound).all()
+
+
+@pytest.mark.gpu
+def test_shared_scratch_in_one_graph():
+    """A packed call and a batch over the same 4-bit cache, both sharing keys and so
+    the cache's scratch, one after the other in one graph: every replay has the eager
+    calls' bits, other calls on the cache in between."""
+    n_head, n_kv, hd, n = 2, 1, 128, 2600
+    shape = dict(n_head=n_head, n_kv=n_kv, head_dim=hd, scale=hd**-0.5)
+    q, k, v = rows_of(1, n, n_head * hd), rows_of(2, n, n_kv * hd), rows_of(3, n, n_kv * hd)
+    starts = [0, 2000, n]
+    dev = [hip_rt.malloc(x.nbytes) for x in (q, k, v, q, q)]
+    try:
+        with nh.KVCache([4096], [n_kv * hd], q4=True) as kv:
+            for d, x in zip(dev, (q, k, v)):
+                hip_rt.to_device(d, x)
+            kv.append_f32(0, 0, k, v)
+
+            def both():
+                kv.attend_packed_device(*dev[:4], starts=starts, bf16=False, **shape)
+                kv.attend_device(0, dev[0], dev[4], n_tok=30, pos0=n - 30, n_seq=n, window=0, causal=True, **shape)
+
+            def outs():
+                kv.sync()
+                return hip_rt.to_host(np.empty_like(q), dev[3]), hip_rt.to_host(np.empty_like(q[:30]), dev[4])
+
+            both()
+            want = outs()
+            graph = hip_rt.Graph(kv.stream, both)
+            for i in range(4):
+                hip_rt.to_device(dev[3], np.zeros_like(q))
+                graph.launch(kv.stream)
+                for a, b in zip(outs(), want):
+                    assert np.array_equal(a, b), i
+                kv.attend(0, q[:20 + i], pos0=n - 20 - i, n_seq=n, **shape)
+            graph.close()
+    finally:
+        for d in dev:
+            hip_rt.free(d)

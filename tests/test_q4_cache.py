@@ -432,3 +432,37 @@ def test_positions_past_the_limit():
             with pytest.raises(nh.NncError) as e:
                 kv.attend(0, q, **{**shape, "n_seq": far + 30, **bad})
             assert e.value.status == nh.NncStatus.INVALID_ARGUMENT
+
+
+CORNERS = [  # n_head, n_kv, head_dim, rows, n_seq, pos0, n_tok, window, causal
+    (16, 1, 512, 1024, 900, 899, 1, 0, True),
+    (16, 1, 512, 1024, 900, 862, 38, 0, True),
+    (16, 1, 192, 2048, 1999, 1998, 1, 0, True),
+    (32, 2, 128, 4096, 4000, 3984, 16, 0, True),  # 256 pairs a KV head
+    (11, 1, 32, 8192, 8000, 7999, 1, 0, True),
+    (33, 11, 32, 96, 90, 80, 10, 1, True),  # every token its own key alone
+    (8, 2, 64, 512, 300, 400, 3, 0, True),  # positions past the last key
+    (8, 2, 64, 512, 300, 400, 30, 0, True),
+    (8, 2, 64, 512, 300, 280, 60, 25, True),  # the last tokens see nothing
+    (8, 2, 96, 512, 300, 285, 14, 7, False),
+    (1, 1, 256, 64, 40, 0, 40, 2, False),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_head,n_kv,hd,rows,n_seq,pos0,n_tok,window,causal", CORNERS)
+def test_corners(n_head, n_kv, hd, rows, n_seq, pos0, n_tok, window, causal):
+    """The largest groups and heads, the narrowest windows, positions past the last
+    key; in exact mode every token has its one-token bits."""
+    print(f"corner {n_head}/{n_kv}/{hd} rows {rows} n_seq {n_seq} tokens {pos0}+{n_tok} window {window}", flush=True)
+    shape = dict(n_seq=n_seq, window=window, causal=causal, n_head=n_head, n_kv=n_kv, head_dim=hd, scale=hd**-0.5)
+    q = rows_of(9, n_tok, n_head * hd)
+    kv, k, v = filled(n_seq, n_kv * hd, rows)
+    with kv:
+        got = kv.attend(0, q, pos0=pos0, **shape)
+        want, bound, _ = ref.attend(q, k, v, pos0=pos0, **shape)
+        assert (np.abs(got - want) <= bound).all()
+        kv.set_exact_batches(True)
+        exact = kv.attend(0, q, pos0=pos0, **shape)
+        for t in sorted({0, n_tok // 2, n_tok - 1}):
+            assert np.array_equal(exact[t:t + 1], kv.attend(0, q[t:t + 1], pos0=pos0 + t, **shape)), t
