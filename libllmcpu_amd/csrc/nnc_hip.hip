@@ -177,6 +177,7 @@ namespace
 struct nnc_hip_kv
 {
 	int device = 0;
+	bool several_devices = false;
 	int n_cu = 256;
 	bool bf16 = true;
 	bool q4 = false; // a 4-bit cache (bf16 is false)
@@ -349,12 +350,14 @@ namespace
 		return NNC_OK;
 	}
 
-	// Makes a cache's device current for a call's launches and allocations.
+	// Makes a cache's device current for a call's launches and allocations (asked
+	// for only where there are several: a call's issue is 0.1 us longer for it).
 	class device_scope
 	{
 	public:
-		explicit device_scope(int device) : want_(device)
+		explicit device_scope(const nnc_hip_kv* kv) : want_(kv->device), was_(kv->device)
 		{
+			if (!kv->several_devices) return;
 			if (hipGetDevice(&was_) != hipSuccess || was_ == want_) was_ = want_;
 			else (void)hipSetDevice(want_);
 		}
@@ -366,7 +369,7 @@ namespace
 		device_scope& operator=(const device_scope&) = delete;
 
 	private:
-		int want_, was_ = 0;
+		int want_, was_;
 	};
 
 	const char* kind_name(const nnc_hip_kv* kv) { return kv->q4 ? "4-bit" : kv->bf16 ? "BF16" : "F32"; }
@@ -424,7 +427,7 @@ namespace
 	// not all be finite is refused: no kernel looks for such values.
 	nnc_status append_raw_q4(nnc_hip_kv* kv, int32_t buf, int32_t pos0, int32_t n_tok, const void* k_rows, const void* v_rows)
 	{
-		const device_scope on(kv->device);
+		const device_scope on(kv);
 		const kv_buffer& b = kv->bufs[buf];
 		const size_t blocks = static_cast<size_t>(b.kv_dim / nnchip::kQ4Block), bytes = blocks * n_tok * nnchip::kQ4RawBlock;
 		for (const void* rows : {k_rows, v_rows})
@@ -810,7 +813,7 @@ namespace
 	                       int32_t n_seq, int32_t window, bool causal, int32_t n_head, int32_t n_kv, int32_t head_dim,
 	                       float scale, const part_source& src = part_source{})
 	{
-		const device_scope on(kv->device);
+		const device_scope on(kv);
 		const kv_buffer& b = kv->bufs[buf];
 		const int group = n_head / n_kv;
 		const bool bf16 = kv->bf16;
@@ -1011,6 +1014,7 @@ namespace
 		if (!kv) return fail(NNC_ERR_OUT_OF_MEMORY, "out of host memory");
 		kv->bf16 = bf16;
 		kv->q4 = q4;
+		kv->several_devices = n_dev > 1;
 		auto bail = [&](nnc_status s)
 		{
 			release(kv);
@@ -1139,6 +1143,7 @@ nnc_status nnc_hip_kv_append_f32(nnc_hip_kv* kv, int32_t buf, int32_t pos0, int3
                                  const float* v_rows)
 {
 	if (nnc_status s = check_append(kv, buf, pos0, n_tok, k_rows, v_rows)) return s;
+	const device_scope on(kv);
 	const size_t bytes = static_cast<size_t>(n_tok) * kv->bufs[buf].kv_dim * sizeof(float);
 	if (nnc_status s = reserve(kv, kv->rows_k, bytes, "append staging")) return s;
 	if (nnc_status s = reserve(kv, kv->rows_v, bytes, "append staging")) return s;
@@ -1157,7 +1162,7 @@ nnc_status nnc_hip_kv_append_f32_device(nnc_hip_kv* kv, int32_t buf, int32_t pos
                                         const float* v_rows)
 {
 	if (nnc_status s = check_append(kv, buf, pos0, n_tok, k_rows, v_rows)) return s;
-	const device_scope on(kv->device);
+	const device_scope on(kv);
 	const kv_buffer& b = kv->bufs[buf];
 	if (kv->q4)
 	{
@@ -1217,7 +1222,7 @@ nnc_status nnc_hip_kv_prep_append_device(nnc_hip_kv* kv, int32_t buf, int32_t po
 	p.eps = pr.rms_eps;
 	p.inv_dim = 1.0f / static_cast<float>(pr.head_dim); // (reference nn_ops.cpp:594)
 	p.rope_cs = nullptr;
-	const device_scope on(kv->device);
+	const device_scope on(kv);
 	if (kv->q4)
 	{
 		// K and V normalised and rotated into F32 rows 0 .. n_tok - 1, quantised from there
@@ -1247,7 +1252,7 @@ nnc_status nnc_hip_kv_read(nnc_hip_kv* kv, int32_t buf, int32_t row0, int32_t n_
 	if (kv->q4)
 	{
 		// through device rows in the interchange form
-		const device_scope on(kv->device);
+		const device_scope on(kv);
 		const size_t bytes = static_cast<size_t>(n_rows) * (b.kv_dim / nnchip::kQ4Block) * nnchip::kQ4RawBlock;
 		if (n_rows == 0 || (!k_out && !v_out)) return nnc_hip_kv_sync(kv);
 		if (nnc_status s = reserve(kv, kv->rows_k, bytes, "K/V read")) return s;
@@ -1279,7 +1284,7 @@ nnc_status nnc_hip_kv_read_f32_device(nnc_hip_kv* kv, int32_t buf, int32_t row0,
 	if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15)
 		return fail(NNC_ERR_INVALID_ARGUMENT, "outputs must be 16-byte aligned");
 	if (n_rows == 0 || (!k_out && !v_out)) return NNC_OK;
-	const device_scope on(kv->device);
+	const device_scope on(kv);
 	if (kv->q4)
 		nnchip::launch_read_q4(b.k, k_out, v_out, b.kv_dim, row0, n_rows, false, kv->stream);
 	else
@@ -1303,6 +1308,7 @@ namespace
 		if (nnc_status s = check_attend(kv, buf, q ? aligned_probe : nullptr, out ? aligned_probe : nullptr, n_tok,
 		                                pos0, n_seq, window, causal, n_head, n_kv, head_dim))
 			return s;
+		const device_scope on(kv);
 		const size_t n = static_cast<size_t>(n_tok) * n_head * head_dim, bytes = n * sizeof(float);
 		const size_t slot = (bytes + 255) & ~static_cast<size_t>(255);
 		if (nnc_status s = reserve(kv, kv->q, bytes, "q staging")) return s;
@@ -1453,7 +1459,7 @@ nnc_status nnc_hip_attend_packed_device(nnc_hip_kv* kv, int32_t type, const void
 	p.causal = causal ? 1 : 0;
 	p.window = window;
 	p.scale = scale;
-	const device_scope on(kv->device);
+	const device_scope on(kv);
 	for (size_t at = 0; at < order.size();)
 	{
 		nnchip::flash_seqs<nnchip::kFlashSeqs> s{};
