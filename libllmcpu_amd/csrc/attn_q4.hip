@@ -450,10 +450,13 @@ namespace nnchip
 					{
 						const float now = up ? m - kBelow : m_off[i];
 						const float f = up ? fast_exp2(m_off[i] - now) : 1.0f;
-						m_off[i] = now;
-						l[i] *= f;
+						if (!__all(m_off[i] == -INFINITY)) // (else nothing has been added yet)
+						{
+							l[i] *= f;
 #pragma unroll
-						for (int b = 0; b < NB; ++b) o[i][b][0] *= f, o[i][b][1] *= f;
+							for (int b = 0; b < NB; ++b) o[i][b][0] *= f, o[i][b][1] *= f;
+						}
+						m_off[i] = now;
 					}
 					const float off = m_off[i] == -INFINITY ? 0.0f : m_off[i];
 #pragma unroll
@@ -778,10 +781,13 @@ namespace nnchip
 						{
 							const float to = up ? m - kBelow : m_off;
 							const float f = up ? fast_exp2(m_off - to) : 1.0f;
-							m_off = to;
-							l *= f;
+							if (!__all(m_off == -INFINITY)) // (else nothing has been added yet)
+							{
+								l *= f;
 #pragma unroll
-							for (int b = 0; b < NB; ++b) oh[b][0] *= f, oh[b][1] *= f, ol[b][0] *= f, ol[b][1] *= f;
+								for (int b = 0; b < NB; ++b) oh[b][0] *= f, oh[b][1] *= f, ol[b][0] *= f, ol[b][1] *= f;
+							}
+							m_off = to;
 						}
 						const float off = m_off == -INFINITY ? 0.0f : m_off;
 #pragma unroll
