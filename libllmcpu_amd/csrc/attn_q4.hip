@@ -307,10 +307,10 @@ namespace nnchip
 		}
 
 		// Two wavefronts per SIMD where their registers fit (256 each).
-		constexpr int q4_per_simd(int nb, int t) { return nb <= 4 && nb * t <= 6 ? 2 : 1; }
+		constexpr int q4_per_simd(int nb) { return nb <= 4 ? 2 : 1; }
 
 		template <int NB, int T, bool FUSE>
-		__global__ __launch_bounds__(64 * kW, q4_per_simd(NB, T)) void decode_q4_kernel(
+		__global__ __launch_bounds__(64 * kW, q4_per_simd(NB)) void decode_q4_kernel(
 			const decode_params p, int group)
 		{
 			constexpr int HD = NB * kQ4Block;
@@ -850,17 +850,27 @@ namespace nnchip
 		}
 
 		template <int NB>
-		void launch_nb(const decode_params& p, int n_tok, int group, hipStream_t stream)
+		void launch_nb(const decode_params& p, int n_tok, int group, int n_cu, hipStream_t stream)
 		{
-			// Up to 8 pairs a wavefront takes them all, up to 16 two tiles of 8 (or, where
-			// their registers do not fit, two work-groups); above that the kernel for
-			// many, whose registers do not fit at 16 blocks.
+			// Up to 8 pairs a wavefront takes them all; up to 16 two tiles of 8, from four
+			// blocks on a work-group each (two tiles' registers leave one wavefront per SIMD
+			// there: 4 tokens of 32 over 8 x 128 at 8k keys 21.1 us alone and 15.5 with three
+			// streams, two work-groups 18.0 and 10.9; of 8 x 64 at 20k 15.0 and 7.6, two
+			// work-groups 15.6 and 8.1). More pairs: a work-group per tile while all of them
+			// are resident at once, else the kernel for many, which makes every value once
+			// (alone / three streams, many -> a work-group per tile: 16 tokens of 4 over 1 x
+			// 256 at 1k keys, 72 work-groups, 26.0 / 8.9 -> 11.5 / 7.1; 6 of 32 over 8 x 128
+			// at 2k, 408, 13.3 / 7.1 -> 10.5 / 6.6; past them 16 of 4 over 1 x 256 at 8k, 504
+			// at one wavefront per SIMD, 30 / 11.5 -> 24 / 17.8; 5 of 32 over 8 x 128 at 9k,
+			// 864, 22.0 / 10.3 -> 18.8 / 11.8). Its registers do not fit at 16 blocks.
 			const int pairs = n_tok * group, tiles = (pairs + 7) / 8;
+			const bool tiled = pairs <= 8 || (NB > 3 && pairs <= 16) || NB > 8 ||
+			                   (pairs > 16 && static_cast<long long>(p.n_split) * p.n_kv * tiles <= q4_per_simd(NB) * n_cu);
 			const dim3 threads(64 * kW);
 			if constexpr (NB <= 8)
-				if (pairs > 16)
+				if (pairs > 16 && !tiled)
 					decode_q4_multi_kernel<NB><<<dim3(p.n_split, p.n_kv, (pairs + 16 * kW - 1) / (16 * kW)), threads, 0, stream>>>(p, group);
-			if constexpr (NB <= 4)
+			if constexpr (NB <= 3)
 				if (pairs > 8 && pairs <= 16)
 					decode_q4_kernel<NB, 2, false><<<dim3(p.n_split, p.n_kv, 1), threads, 0, stream>>>(p, group);
 			if constexpr (NB <= 8)
@@ -869,24 +879,24 @@ namespace nnchip
 					decode_q4_kernel<NB, 1, true><<<dim3(p.n_split, p.n_kv, 1), threads, 0, stream>>>(p, group);
 					return;
 				}
-			if (pairs <= 8 || (NB > 4 && pairs <= 16) || NB > 8)
+			if (tiled)
 				decode_q4_kernel<NB, 1, false><<<dim3(p.n_split, p.n_kv, tiles), threads, 0, stream>>>(p, group);
 			if (p.n_split > 1)
 				merge_q4_kernel<<<dim3(p.n_head, n_tok), kMergeThreads, 0, stream>>>(p, NB * kQ4Block, group);
 		}
 	}
 
-	bool launch_decode_q4(const decode_params& p, int n_tok, int head_dim, int group, hipStream_t stream)
+	bool launch_decode_q4(const decode_params& p, int n_tok, int head_dim, int group, int n_cu, hipStream_t stream)
 	{
 		switch (head_dim)
 		{
-		case 32: launch_nb<1>(p, n_tok, group, stream); return true;
-		case 64: launch_nb<2>(p, n_tok, group, stream); return true;
-		case 96: launch_nb<3>(p, n_tok, group, stream); return true;
-		case 128: launch_nb<4>(p, n_tok, group, stream); return true;
-		case 192: launch_nb<6>(p, n_tok, group, stream); return true;
-		case 256: launch_nb<8>(p, n_tok, group, stream); return true;
-		case 512: launch_nb<16>(p, n_tok, group, stream); return true;
+		case 32: launch_nb<1>(p, n_tok, group, n_cu, stream); return true;
+		case 64: launch_nb<2>(p, n_tok, group, n_cu, stream); return true;
+		case 96: launch_nb<3>(p, n_tok, group, n_cu, stream); return true;
+		case 128: launch_nb<4>(p, n_tok, group, n_cu, stream); return true;
+		case 192: launch_nb<6>(p, n_tok, group, n_cu, stream); return true;
+		case 256: launch_nb<8>(p, n_tok, group, n_cu, stream); return true;
+		case 512: launch_nb<16>(p, n_tok, group, n_cu, stream); return true;
 		default: return false;
 		}
 	}

@@ -137,7 +137,7 @@ namespace nnchip
 		return head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 192 ||
 		       head_dim == 256 || head_dim == 512;
 	}
-	bool launch_decode_q4(const decode_params& p, int n_tok, int head_dim, int group, hipStream_t stream);
+	bool launch_decode_q4(const decode_params& p, int n_tok, int head_dim, int group, int n_cu, hipStream_t stream);
 	// Rows into the records: F32, or (raw) blocks in the interchange form; and
 	// rows row0 .. row0 + n_rows - 1 out of them, likewise. Either output may be
 	// null.

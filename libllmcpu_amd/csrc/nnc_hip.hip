@@ -626,7 +626,7 @@ namespace
 		// One-token launches of the MFMA kernels over a few splits merge in
 		// the split launch; the counts are the cache's, used in stream order.
 		if ((kv->q4 || nnchip::mfma_shape(head_dim, group)) && n_kv <= nnchip::kFuseCounts) p.counts = kv->counts;
-		if (kv->q4 ? !nnchip::launch_decode_q4(p, n_tok, head_dim, group, kv->stream)
+		if (kv->q4 ? !nnchip::launch_decode_q4(p, n_tok, head_dim, group, kv->n_cu, kv->stream)
 		           : !nnchip::launch_decode(p, n_tok, head_dim, group, kv->bf16, kv->stream))
 			return fail(NNC_ERR_UNSUPPORTED_MODEL, "no decode kernel for head_dim %d, group %d", head_dim, group);
 		NNC_HIP_TRY(hipGetLastError(), "decode launch");

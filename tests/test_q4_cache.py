@@ -466,3 +466,22 @@ def test_corners(n_head, n_kv, hd, rows, n_seq, pos0, n_tok, window, causal):
         exact = kv.attend(0, q, pos0=pos0, **shape)
         for t in sorted({0, n_tok // 2, n_tok - 1}):
             assert np.array_equal(exact[t:t + 1], kv.attend(0, q[t:t + 1], pos0=pos0 + t, **shape)), t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_head,n_kv,hd,n_seq,window", [
+    (32, 8, 128, 500, 0), (32, 8, 128, 2000, 0), (32, 8, 128, 9000, 0), (32, 8, 64, 2000, 300), (4, 1, 256, 1000, 0), (4, 1, 256, 8000, 0),
+    (8, 4, 256, 3000, 0), (12, 4, 192, 700, 0), (16, 4, 32, 900, 0), (12, 6, 96, 400, 0), (6, 3, 512, 600, 0)])
+def test_batch_bits_whatever_the_kernel(n_head, n_kv, hd, n_seq, window):
+    """Batches of as many (token, head) pairs as one wavefront, two, a work-group per
+    tile or the kernel for many take."""
+    shape = dict(n_seq=n_seq, window=window, n_head=n_head, n_kv=n_kv, head_dim=hd, scale=hd**-0.5)
+    kv, k, v = filled(n_seq, n_kv * hd, (n_seq + 31) // 32 * 32)
+    q = rows_of(3, 16, n_head * hd)
+    with kv:
+        one = [kv.attend(0, q[t:t + 1], pos0=n_seq - 16 + t, **shape)[0] for t in range(16)]
+        want, bound, _ = ref.attend(q, k, v, pos0=n_seq - 16, causal=True, **shape)
+        assert (np.abs(np.array(one) - want) <= bound).all()
+        for a, b in ((0, 16), (13, 16), (9, 13), (3, 8), (10, 16), (0, 8), (1, 14), (14, 16)):
+            print(f"bits {n_head}/{n_kv}/{hd} n_seq {n_seq} tokens {a} .. {b}", flush=True)
+            assert np.array_equal(kv.attend(0, q[a:b], pos0=n_seq - 16 + a, **shape), np.array(one[a:b])), (a, b)
