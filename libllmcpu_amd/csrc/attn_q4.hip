@@ -561,8 +561,8 @@ namespace nnchip
 		// modulo kW) follow one another, with sums of their own, and join in the same
 		// order, so a pair gets the same bits. Bound: VALU (the softmax of 16 pairs in
 		// fp16 parts, and every class's sums joined: some 300 operations per group of 32
-		// keys; matrix units 17 % busy) and the partials, as many bytes as the records.
-		// (13 tokens of 32 over 8 x 128 at 20k keys: 21.3 us a call; with the kernel
+		// keys; matrix units 18 % busy) and the partials, written and read as many bytes as
+		// the records. (13 tokens of 32 over 8 x 128 at 20k keys: 20.9 us a call; with the kernel
 		// above, two tiles of 8 pairs per wavefront, every tile's weights computed twice
 		// and every value made four times, 68.)
 		template <int NB>
