@@ -424,7 +424,7 @@ class KVCache:
         q, k, v = (np.ascontiguousarray(x) for x in (q, k, v))
         if q.dtype not in (np.float32, np.uint16) or k.dtype != q.dtype or v.dtype != q.dtype:
             raise ValueError("q, k and v are float32, or uint16 BF16 bits")
-        rows = max(0, *starts)
+        rows = max([0, *starts])
         if q.size < rows * n_head * head_dim or min(k.size, v.size) < rows * n_kv * head_dim:
             raise ValueError(f"q, k or v is shorter than {rows} rows")
         out, dev = np.zeros_like(q), []

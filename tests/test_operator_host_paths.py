@@ -211,7 +211,7 @@ def refusals_launch_nothing(rt, nh):
         rt.clear()
         for change in (dict(starts=[0, 9, 8]), dict(starts=[-1, 9]), dict(window=-1), dict(n_head=5), dict(n_kv=0), dict(head_dim=4),
                        dict(head_dim=264, q_stride=4096, k_stride=4096, v_stride=4096, out_stride=4096), dict(q_stride=248), dict(v_stride=132),
-                       dict(k_stride=1 << 23), dict(starts=[0, 3, (1 << 27)])):
+                       dict(k_stride=1 << 23), dict(starts=[0, 3, (1 << 27)]), dict(starts=[])):
             with pytest.raises(nh.NncError):
                 kv.attend_packed_device(Q, K, V, OUT, **{**ok, **change})
         for a in ((Q + 8, K, V, OUT), (Q, K, V, K), (Q, K, V, V), (0, K, V, OUT), (Q, K, V, 0), (Q, K + 4, V, OUT)):
